@@ -93,6 +93,16 @@ typedef enum {
   RF_ERR_DEVICE = 4        /* a kernel reported an error (see rf_moe_device_status) */
 } rf_status;
 
+typedef enum {
+  RF_SCORE_SOFTMAX = 0,
+  RF_SCORE_SIGMOID = 1
+} rf_scoring;
+
+typedef enum {
+  RF_GROUP_MAX = 0,   /* a group's score is its largest selection score */
+  RF_GROUP_TOP2 = 1   /* the sum of its two largest */
+} rf_group_score;
+
 /* Device-side error codes reported by rf_moe_device_status. */
 #define RF_DEV_OK 0
 #define RF_DEV_BAD_EXPERT_ID 1   /* a routed id was outside [0, E) */
@@ -152,6 +162,34 @@ int rf_moe_router_topk(const void *x, int x_dtype, const void *gate, int gate_dt
                        float *topk_weights, int32_t *topk_ids32, int64_t *topk_ids64,
                        float *logits, void *workspace, size_t workspace_bytes,
                        rf_stream_t stream);
+
+/*
+ * Grouped routing.  Logits as in rf_moe_router_topk (gate, bias, round_dtype,
+ * shared_gate, workspace and the gate == NULL form alike), then per token:
+ *   s = softmax(logit) or sigmoid(logit)                      (scoring)
+ *   c = s + select_bias[e]   (NULL: c = s; chooses, never weighs; -inf closes
+ *                             an expert, +inf and NaN are not meant to be used)
+ *   num_groups > 1: the experts form groups of E / num_groups consecutive ids;
+ *     a group's score is its largest c or the sum of its two largest
+ *     (group_score); the topk_groups best stay, elsewhere c = -inf
+ *   ids = the K largest c in descending order; ties go to the lower id (and
+ *     the lower group); a NaN c counts as -inf, so ids are always valid and
+ *     distinct, and the weights of NaN scores are NaN
+ *   weights = s[ids], / max(sum, 1e-20) when renormalize, * scale
+ * The order is that of the exact scores of the fp32 logits: where fp32 scores
+ * are too close to tell, the token is decided in fp64.
+ * Requires 1 <= K <= min(16, topk_groups * E / num_groups), E <= 1024,
+ * num_groups <= 32 and dividing E; x 16-byte aligned.  No counterpart in the
+ * reference (its router is softmax top-k, moe_layer.py:320-344).
+ */
+int rf_moe_router_grouped_topk(const void *x, int x_dtype, const void *gate, int gate_dtype,
+                               const float *bias, int64_t T, int64_t H, int64_t E, int64_t K,
+                               int scoring, const float *select_bias, int64_t num_groups,
+                               int64_t topk_groups, int group_score, int renormalize, float scale,
+                               int round_dtype, const void *shared_gate, float *shared_scale,
+                               float *topk_weights, int32_t *topk_ids32, int64_t *topk_ids64,
+                               float *logits, void *workspace, size_t workspace_bytes,
+                               rf_stream_t stream);
 
 /*
  * K2 — counting-sort permute of the T*K pairs by expert (stable), plus the
@@ -538,6 +576,75 @@ int rf_moe_combine_rmsnorm(const void *y, const int32_t *row_of_slot, const floa
                            const void *shared_y, const float *shared_scale, const void *residual,
                            int mode, const float *norm_weight, const float *norm_bias, float eps,
                            void *residual_out, void *normed_out, rf_stream_t stream);
+
+/*
+ * 4-bit expert weights with group scales: weight[n, k] = scale[n, k / group] *
+ * (code[n, k] - 8), codes 0..15, group_size 32, 64 or 128 along k, scales in
+ * the layer dtype (RF_BF16 or RF_F16).  N (each half of it when gated: w1's
+ * gate and up rows) and K are multiples of 8; K need not be a multiple of the
+ * group.  The stored layout is the kernels' own (16-row x 64-k blocks);
+ * rf_moe_int4_data_size bytes and rf_moe_int4_scales_count scales per weight
+ * (-1 for sizes that are not served), both 16-byte aligned.
+ *   rf_moe_int4_pack        from codes [S, N, K/2] uint8 (k even in the low
+ *                           four bits, k odd in the high) and scales
+ *                           [S, N, ceil(K / group)]
+ *   rf_moe_int4_quantize    from weights [S, N, K] of any dtype: a group's
+ *                           scale is max|w| / 7 rounded to five significant
+ *                           bits (scale * (code - 8) is then exact in 16
+ *                           bits), its codes the nearest, clamped to 0..15
+ *   rf_moe_int4_dequantize  back to [S, N, K] in the layer dtype
+ */
+int64_t rf_moe_int4_data_size(int64_t S, int64_t N, int64_t K, int64_t group_size, int gated);
+int64_t rf_moe_int4_scales_count(int64_t S, int64_t N, int64_t K, int64_t group_size, int gated);
+int rf_moe_int4_pack(const void *codes, const void *scales, int dtype, int64_t S, int64_t N,
+                     int64_t K, int64_t group_size, int gated, void *data, void *packed_scales,
+                     rf_stream_t stream);
+int rf_moe_int4_quantize(const void *w, int w_dtype, int dtype, int64_t S, int64_t N, int64_t K,
+                         int64_t group_size, int gated, void *data, void *packed_scales,
+                         rf_stream_t stream);
+int rf_moe_int4_dequantize(const void *data, const void *packed_scales, int dtype, int64_t S,
+                           int64_t N, int64_t K, int64_t group_size, int gated, void *w,
+                           rf_stream_t stream);
+
+/*
+ * The routed experts with 4-bit weights, from tokens to tokens (permute, gated
+ * products, down products, combine):
+ *   h = act(x . W1g[e]^T) * (x . W1u[e]^T)     rounded to dtype
+ *   out[t] = round(sum_k w[t,k] (h . W2[e]^T) + shared_scale[t] * shared_y[t]
+ *                  + residual[t])               fp32 up to the rounding
+ * x [T, H], out / shared_y / residual [T, H] in dtype (RF_BF16 or RF_F16);
+ * w1 a gated weight of N = 2I, K = H, w2 one of N = H, K = I, E slots each;
+ * topk_ids outside [0, E) add nothing and set RF_DEV_BAD_EXPERT_ID.
+ * shared_y, shared_scale, residual may be NULL; out may be residual.
+ * workspace: rf_moe_int4_experts_workspace_size bytes, 256-byte aligned.
+ */
+size_t rf_moe_int4_experts_workspace_size(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I);
+int rf_moe_int4_experts(const void *x, int dtype, const void *w1, const void *w1_scales,
+                        int64_t w1_group, const void *w2, const void *w2_scales, int64_t w2_group,
+                        const float *topk_weights, const int32_t *topk_ids, int64_t T, int64_t K,
+                        int64_t E, int64_t H, int64_t I, int activation, const void *shared_y,
+                        const float *shared_scale, const void *residual, void *out,
+                        void *workspace, size_t workspace_bytes, rf_stream_t stream);
+
+/*
+ * Residual addition, RMSNorm (reframework/layers/norm.py:27-53) and an e4m3
+ * output with scales:
+ *   r = round(x + residual) -> residual_out    (residual NULL: r = x, and
+ *                                               residual_out may be NULL)
+ *   z = r / sqrt(mean(r^2) + eps) * norm_weight (+ norm_bias)      fp32
+ *   normed_out = round(z) (NULL to skip)
+ *   per group of group_size columns (0: the row):
+ *     scales = max|z| / 448 (1 for a group of zeros), q = e4m3(z / scale)
+ * q and scales may be NULL together when normed_out is given.
+ * A group with a NaN or an infinity gets scale NaN and zero codes.  x,
+ * residual, residual_out and normed_out [T, H] in dtype; q [T, H] e4m3; scales
+ * [T, H / group_size] (or [T]) fp32.  residual_out may be residual or x;
+ * group_size is 0, 32, 64 or 128 and divides H; a row of up to 65536 bytes.
+ */
+int rf_moe_add_rmsnorm_q8(const void *x, const void *residual, int64_t T, int64_t H, int dtype,
+                          const float *norm_weight, const float *norm_bias, float eps,
+                          int64_t group_size, void *residual_out, void *normed_out, void *q,
+                          float *scales, rf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,8 @@ LIB_PATH = os.path.join(_HERE, "_rf_moe.so")
 
 RF_F32, RF_F16, RF_BF16 = 0, 1, 2
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
 COMBINE_REFERENCE, COMBINE_FP32 = 0, 1
 DEV_ERRORS = {0: "ok", 1: "routed expert id out of range", 2: "pipeline wait timed out",
               3: "expert-parallel plan exceeds its buffers"}
@@ -103,6 +105,23 @@ _SIGNATURES = {
                                                                                  ctypes.c_int32] + [_c_void_p] * 5),
     "rf_moe_split_combine": (_int, [_c_void_p] * 6 + [_i64, ctypes.c_int32, _i64, ctypes.c_int32, ctypes.c_int32,
                                                        _c_void_p, _c_void_p]),
+    "rf_moe_router_grouped_topk": (_int, [_c_void_p, _int, _c_void_p, _int, _c_void_p, _i64, _i64, _i64, _i64, _int,
+                                          _c_void_p, _i64, _i64, _int, _int, ctypes.c_float, _int, _c_void_p, _c_void_p,
+                                          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t,
+                                          _c_void_p]),
+    "rf_moe_int4_data_size": (_i64, [_i64, _i64, _i64, _i64, _int]),
+    "rf_moe_int4_scales_count": (_i64, [_i64, _i64, _i64, _i64, _int]),
+    "rf_moe_int4_pack": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _int, _c_void_p, _c_void_p,
+                                _c_void_p]),
+    "rf_moe_int4_quantize": (_int, [_c_void_p, _int, _int, _i64, _i64, _i64, _i64, _int, _c_void_p, _c_void_p,
+                                    _c_void_p]),
+    "rf_moe_int4_dequantize": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64, _int, _c_void_p, _c_void_p]),
+    "rf_moe_int4_experts_workspace_size": (ctypes.c_size_t, [_i64] * 5),
+    "rf_moe_int4_experts": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p,
+                                   _c_void_p, _i64, _i64, _i64, _i64, _i64, _int, _c_void_p, _c_void_p, _c_void_p,
+                                   _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p]),
+    "rf_moe_add_rmsnorm_q8": (_int, [_c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _c_void_p, ctypes.c_float, _i64,
+                                     _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "rf_moe_ep_plan": (_int, [_c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _c_void_p, _c_void_p,
                               ctypes.c_int32, ctypes.c_int32, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }

@@ -1,0 +1,73 @@
+// 4-bit expert weights with group scales: the stored layout and the device
+// code that turns codes into 16-bit values.
+//
+// A weight is scale[n, k / g] * (code[n, k] - 8), code in 0..15, g in
+// {32, 64, 128} along the reduction axis.  Stored per expert slot:
+//   data   [row blocks][k blocks][512 bytes]   16 rows x 64 k to a block
+//   scales [row blocks][groups][16]            in the layer dtype
+// so that a warp reads a block as 32 consecutive 16-byte words.  Lane
+// 4 * r + c (r = 0..7, c = 0..3) holds, as four 32-bit words of 8 codes: row
+// r's k = 8 c .. 8 c + 7, its k = 32 + 8 c .. 32 + 8 c + 7, and the same of row
+// r + 8.  Those are the rows and, with k renamed the same way for the other
+// operand, the k of the lane's fragments of two 16 x 16 tiles of mma.sync per
+// half of the block (a scale group of 32 is a half), and four 16-byte pieces
+// of a K-major shared-memory tile.  In a word, code 2 i sits in nibble i and
+// code 2 i + 1 in nibble i + 4, so that one shift and one mask give the
+// neighbouring pair as two 16-bit halves.  The scales of rows r and r + 8 are
+// neighbours (entry 2 r + h).
+// Rows and k past the weight's own are stored as code 8 (zero) with scale 0;
+// a gated weight's gate and up halves are padded to whole row blocks each.
+#pragma once
+
+#include "common.cuh"
+
+namespace rf {
+
+constexpr int I4_ROWS = 16, I4_K = 64, I4_BLOCK = 512;
+
+struct Int4Shape {
+  int64_t half_rows;   // rows of one half (N, or N / 2 gated)
+  int halves;          // 2 gated, 1 otherwise
+  int64_t half_blocks; // row blocks of one half
+  int64_t k_blocks;
+  int64_t groups;      // scale groups along K
+
+  __host__ __device__ int64_t row_blocks() const { return half_blocks * halves; }
+  __host__ __device__ int64_t slot_bytes() const { return row_blocks() * k_blocks * I4_BLOCK; }
+  __host__ __device__ int64_t slot_scales() const { return row_blocks() * groups * I4_ROWS; }
+};
+
+inline __host__ __device__ Int4Shape int4_shape(int64_t N, int64_t K, int64_t group, bool gated) {
+  Int4Shape s;
+  s.halves = gated ? 2 : 1;
+  s.half_rows = N / s.halves;
+  s.half_blocks = (s.half_rows + I4_ROWS - 1) / I4_ROWS;
+  s.k_blocks = (K + I4_K - 1) / I4_K;
+  s.groups = (K + group - 1) / group;
+  return s;
+}
+
+// Sizes, group and dtype of a 4-bit weight that the kernels take.
+inline bool int4_valid(int64_t N, int64_t K, int64_t group, bool gated) {
+  return N > 0 && K > 0 && K % 8 == 0 && (N / (gated ? 2 : 1)) % 8 == 0 && (!gated || N % 2 == 0) &&
+         (group == 32 || group == 64 || group == 128) && N < ((int64_t)1 << 30) && K < ((int64_t)1 << 30);
+}
+
+// The pair of codes (2 i, 2 i + 1) of a word as two 16-bit values code - 8,
+// exact: code | 128.0 (bf16) or code | 1024.0 (fp16) has the code in its last
+// mantissa bits, and subtracting 136 or 1032 leaves code - 8.
+template <typename T> __device__ __forceinline__ uint32_t int4_pair(uint32_t word, int i);
+template <> __device__ __forceinline__ uint32_t int4_pair<__nv_bfloat16>(uint32_t word, int i) {
+  const uint32_t b = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 off = __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));  // 136
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&b), off);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t int4_pair<__half>(uint32_t word, int i) {
+  const uint32_t b = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+  const __half2 off = __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1032
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+}  // namespace rf

@@ -1,0 +1,241 @@
+// Residual addition + RMSNorm + e4m3 output with scales, one pass over the rows.
+//
+// Per row (reframework/layers/norm.py:27-53 up to the last step):
+//   r = round(x + residual)                 in the layer dtype (r = x without a residual)
+//   z = r * 1/sqrt(mean(r^2) + eps) * w (+ b)   in fp32, on the stored r
+//   per group of g columns (g = H: the whole row):
+//     scale = max|z| / 448, q = e4m3(z / scale)   (448: the largest e4m3)
+// An all-zero group has scale 1; a group holding a NaN or an infinity has
+// scale NaN and zero codes, so that every value it stands for is NaN.
+//
+// HBM-bound: each input element is read once and kept in registers across the
+// two reductions (sum of squares, then max|z|), each output written once.  The
+// sums and z are fp32; the roundings are those of the outputs' types.  A row
+// belongs to one warp (up to 128 16-byte vectors) or to one block; the threads
+// keep their columns' weights in registers over all rows that they take.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+RF_DEVICE_ERROR_WORD();
+
+namespace {
+
+constexpr float E4M3_MAX = 448.0f;
+constexpr float MIN_SCALE = 0x1p-126f;  // keeps 1 / scale finite
+constexpr unsigned FULL = 0xffffffffu;
+
+struct NormArgs {
+  const void *x;
+  const void *residual;  // may be NULL
+  const float *w;
+  const float *b;        // may be NULL
+  void *residual_out;    // may be NULL without a residual
+  void *normed;          // may be NULL
+  uint8_t *q;            // [T, H] e4m3; may be NULL (then so is scales)
+  float *scales;         // [T, H / g]
+  int64_t T;
+  int H;
+  int lanes;             // threads that share a group: g / V (0: the whole row)
+  int n_groups;          // H / g
+  float eps;
+};
+
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  if constexpr (TPR > 32) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) v += red[w];
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ float row_max(float v, float *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  if constexpr (TPR > 32) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < TPR / 32; ++w) v = fmaxf(v, red[w]);
+  }
+  return v;
+}
+
+// max|z| of a group -> its scale; a non-finite value was turned into +inf.
+__device__ __forceinline__ float scale_of(float amax) {
+  if (amax == 0.f) return 1.f;
+  if (!(amax < INFINITY)) return NAN;
+  return fmaxf(amax / E4M3_MAX, MIN_SCALE);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T *p, const float *f) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(rf::pack2<T>(f[0], f[1]), rf::pack2<T>(f[2], f[3]), rf::pack2<T>(f[4], f[5]), rf::pack2<T>(f[6], f[7]));
+  }
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(const float *z, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(z[0] * inv, z[1] * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z[2] * inv, z[3] * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+// TPR threads per row, VPT 16-byte vectors per thread; a warp-row block holds
+// ROWS rows.
+template <typename T, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) add_rmsnorm_q8_kernel(const NormArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int ROWS = TPR == 32 ? 8 : 1;
+  __shared__ float red[TPR / 32];
+  const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  const int nvec = a.H / V;
+  float w[VPT][V];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    const int v = tid + u * TPR;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[u][i] = v < nvec ? a.w[v * V + i] : 0.f;
+  }
+  const T *x = reinterpret_cast<const T *>(a.x);
+  const T *res = reinterpret_cast<const T *>(a.residual);
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  for (int64_t t = (int64_t)blockIdx.x * ROWS + (TPR == 32 ? threadIdx.x >> 5 : 0); t < a.T; t += step) {
+    float z[VPT][V];
+    float ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int v = tid + u * TPR;
+      const bool ok = v < nvec;
+      const int64_t at = t * a.H + (int64_t)v * V;
+      rf::unpack16<T>(ok ? __ldg(reinterpret_cast<const uint4 *>(x + at)) : make_uint4(0u, 0u, 0u, 0u), z[u]);
+      if (res) {
+        float f[V];
+        rf::unpack16<T>(ok ? __ldg(reinterpret_cast<const uint4 *>(res + at)) : make_uint4(0u, 0u, 0u, 0u), f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[u][i] = rf::round_to<T>(__fadd_rn(z[u][i], f[i]));
+      }
+      if (a.residual_out && ok) store_vec<T, V>(reinterpret_cast<T *>(a.residual_out) + at, z[u]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) ss = fmaf(z[u][i], z[u][i], ss);
+    }
+    const float inv = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.H + a.eps);
+    float amax = 0.f;  // of this thread's columns (the whole row is one group)
+    float vmax[VPT];   // of one vector
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int v = tid + u * TPR;
+      vmax[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        z[u][i] = z[u][i] * inv * w[u][i];
+        if (a.b && v < nvec) z[u][i] += a.b[v * V + i];
+        // a NaN counts as an infinity (fmaxf would drop it); lanes past the row hold 0 * inv
+        const float m = v < nvec ? fabsf(z[u][i]) : 0.f;
+        vmax[u] = fmaxf(vmax[u], m == m ? m : INFINITY);
+      }
+      amax = fmaxf(amax, vmax[u]);
+    }
+    if (a.lanes == 0) {
+      amax = row_max<TPR>(amax, red);
+#pragma unroll
+      for (int u = 0; u < VPT; ++u) vmax[u] = amax;
+      if (tid == 0 && a.q) a.scales[t] = scale_of(amax);
+    } else {
+#pragma unroll
+      for (int u = 0; u < VPT; ++u) {
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) vmax[u] = fmaxf(vmax[u], __shfl_xor_sync(FULL, vmax[u], o));
+        const int v = tid + u * TPR;
+        if (v < nvec && v % a.lanes == 0 && a.q) a.scales[t * a.n_groups + v / a.lanes] = scale_of(vmax[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int v = tid + u * TPR;
+      if (v >= nvec) continue;
+      const int64_t at = t * a.H + (int64_t)v * V;
+      if (a.normed) store_vec<T, V>(reinterpret_cast<T *>(a.normed) + at, z[u]);
+      if (!a.q) continue;
+      const float scale = scale_of(vmax[u]);
+      const bool fine = scale == scale;
+      const float is = 1.0f / scale;
+      uint32_t q[V / 4];
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) q[i] = fine ? e4m3x4(z[u] + 4 * i, is) : 0u;
+      if constexpr (V == 8) *reinterpret_cast<uint2 *>(a.q + at) = make_uint2(q[0], q[1]);
+      else *reinterpret_cast<uint32_t *>(a.q + at) = q[0];
+    }
+  }
+}
+
+template <typename T, int TPR, int VPT>
+int launch_v(const NormArgs &a, cudaStream_t st) {
+  constexpr int ROWS = TPR == 32 ? 8 : 1;
+  constexpr int THREADS = TPR == 32 ? 256 : TPR;
+  const int64_t blocks = std::min<int64_t>((a.T + ROWS - 1) / ROWS, (int64_t)rf::num_sms() * (2048 / THREADS));
+  add_rmsnorm_q8_kernel<T, TPR, VPT><<<(int)blocks, THREADS, 0, st>>>(a);
+  return rf::check_launch("rf_moe_add_rmsnorm_q8");
+}
+
+template <typename T>
+int launch_t(const NormArgs &a, cudaStream_t st) {
+  const int nvec = a.H / (16 / (int)sizeof(T));
+  if (nvec <= 32) return launch_v<T, 32, 1>(a, st);
+  if (nvec <= 64) return launch_v<T, 32, 2>(a, st);
+  if (nvec <= 128) return launch_v<T, 128, 1>(a, st);
+  if (nvec <= 256) return launch_v<T, 256, 1>(a, st);
+  if (nvec <= 512) return launch_v<T, 256, 2>(a, st);
+  if (nvec <= 1024) return launch_v<T, 512, 2>(a, st);
+  if (nvec <= 2048) return launch_v<T, 1024, 2>(a, st);
+  if (nvec <= 4096) return launch_v<T, 1024, 4>(a, st);
+  return rf::fail(RF_ERR_UNSUPPORTED, "rf_moe_add_rmsnorm_q8: a row holds at most 65536 bytes");
+}
+
+}  // namespace
+
+extern "C" int rf_moe_add_rmsnorm_q8(const void *x, const void *residual, int64_t T, int64_t H, int dtype,
+                                     const float *norm_weight, const float *norm_bias, float eps,
+                                     int64_t group_size, void *residual_out, void *normed_out, void *q,
+                                     float *scales, rf_stream_t stream) {
+  RF_CHECK_ARG(rf::valid_dtype(dtype), "rf_moe_add_rmsnorm_q8: unknown dtype");
+  RF_CHECK_ARG(T >= 0 && H > 0 && H < ((int64_t)1 << 30), "rf_moe_add_rmsnorm_q8: bad sizes");
+  const int64_t esz = (int64_t)rf::dtype_size(dtype);
+  RF_CHECK_ARG((H * esz) % 16 == 0, "rf_moe_add_rmsnorm_q8: H * element size must be a multiple of 16 bytes");
+  RF_CHECK_ARG(eps >= 0.f, "rf_moe_add_rmsnorm_q8: eps must be >= 0");
+  RF_CHECK_ARG(group_size == 0 || ((group_size == 32 || group_size == 64 || group_size == 128) && H % group_size == 0),
+               "rf_moe_add_rmsnorm_q8: group_size must be 0 (the row), 32, 64 or 128 and divide H");
+  if (H * esz > 65536) return rf::fail(RF_ERR_UNSUPPORTED, "rf_moe_add_rmsnorm_q8: a row holds at most 65536 bytes");
+  RF_CHECK_ARG(T == 0 || (x && norm_weight && !q == !scales && (q || normed_out) && (residual_out || !residual)),
+               "rf_moe_add_rmsnorm_q8: null pointer");
+  RF_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)residual % 16 == 0 && (uintptr_t)residual_out % 16 == 0 &&
+                   (uintptr_t)normed_out % 16 == 0 && (uintptr_t)q % 16 == 0,
+               "rf_moe_add_rmsnorm_q8: buffers must be 16-byte aligned");
+  RF_CHECK_ARG(T == 0 || ((!q || (q != residual_out && q != normed_out)) && (!normed_out || normed_out != residual_out)),
+               "rf_moe_add_rmsnorm_q8: the outputs must not alias");
+  if (T == 0) return RF_OK;
+  NormArgs a{x, residual, norm_weight, norm_bias, residual_out, normed_out, (uint8_t *)q, scales, T, (int)H, 0, 1, eps};
+  if (group_size) {
+    a.lanes = (int)(group_size * esz / 16);
+    a.n_groups = (int)(H / group_size);
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case RF_F32: return launch_t<float>(a, st);
+    case RF_F16: return launch_t<__half>(a, st);
+    default: return launch_t<__nv_bfloat16>(a, st);
+  }
+}

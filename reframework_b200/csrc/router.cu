@@ -27,22 +27,17 @@
 //       order (deterministic), applies rounding / bias, softmax, top-k,
 //       renormalisation or the entropy-adaptive rule, writes weights and ids.
 // The shared-expert gate (sigmoid(x . w_s)) is one more "expert" column.
-#include "gemm.cuh"
+#include "router.cuh"
 
 RF_DEVICE_ERROR_WORD();
 
 namespace {
 
+using rf::round_dt;
+using rf::sum_slices;
+constexpr int KMAX = rf::ROUTER_KMAX;
 constexpr int THREADS = 256;
 constexpr int SLICE = 256;     // H elements per slice: fixed, so the sum order never depends on T
-constexpr int KMAX = 16;
-
-__device__ __forceinline__ float round_dt(int dtype, float v) {
-  if (dtype == RF_BF16) return __bfloat162float(__float2bfloat16_rn(v));
-  if (dtype == RF_F16) return __half2float(__float2half_rn(v));
-  return v;
-}
-
 struct LogitsArgs {
   const void *x;
   const void *gate;
@@ -228,21 +223,6 @@ __device__ __forceinline__ float load_logit(const TopkArgs &a, int64_t t, int e)
 
 constexpr int TK_WARPS = 8;
 
-// 0 + p[0] + p[stride] + ... in slice order, eight loads in flight at a time.
-__device__ __forceinline__ float sum_slices(const float *p, int64_t stride, int n) {
-  float v = 0.f;
-  int z = 0;
-  for (; z + 8 <= n; z += 8) {
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = p[(int64_t)(z + i) * stride];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v += q[i];
-  }
-  for (; z < n; ++z) v += p[(int64_t)z * stride];
-  return v;
-}
-
 template <typename TX>
 __global__ void __launch_bounds__(TK_WARPS * 32) router_topk_kernel(TopkArgs a) {
   extern __shared__ float s_lg[];  // [TK_WARPS][E]
@@ -387,6 +367,50 @@ void launch_logits_tg(const LogitsArgs &a, const Plan &p, int gate_dtype, cudaSt
 
 }  // namespace
 
+namespace rf {
+
+int router_logits(const char *what, const void *x, int x_dtype, const void *gate, int gate_dtype,
+                  const void *shared_gate, int64_t T, int64_t H, int64_t E, void *workspace,
+                  size_t workspace_bytes, cudaStream_t st, RouterLogits *out) {
+  const int Ec = (int)E + (shared_gate ? 1 : 0);
+  const Plan p = make_plan(T, (int)H, Ec);
+  const size_t need = (size_t)p.slices * (size_t)T * (size_t)Ec * sizeof(float);
+  RF_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0,
+               std::string(what) + ": workspace too small (see rf_moe_router_workspace_size)");
+  RF_CHECK_ARG(p.ttiles <= 0x7fffffff && p.slices <= 65535, std::string(what) + ": too many tokens");
+  // Tensor cores when x and the gate share a 16-bit dtype and the shared
+  // gate (if any) is the row right after the gate's E rows: one tile per
+  // (128 tokens, slice of H), each slice a fixed MMA sequence, partials
+  // [slices][T][ld] summed in slice order by the top-k pass (the same bits
+  // whatever T is; few tokens still get one CTA per slice).  Otherwise the
+  // CUDA-core slices.
+  const size_t esz = (size_t)rf::dtype_size(gate_dtype);
+  const bool adjacent = !shared_gate ||
+                        (const char *)shared_gate == (const char *)gate + (size_t)E * (size_t)H * esz;
+  const int64_t ld = (Ec + 3) / 4 * 4;
+  out->partial = reinterpret_cast<const float *>(workspace);
+  out->slices = p.slices;
+  int rc = -1;
+  if (x_dtype == gate_dtype && adjacent &&
+      workspace_bytes >= (size_t)p.slices * (size_t)T * (size_t)ld * sizeof(float))
+    rc = rf::tc_dense_f32(x, gate, reinterpret_cast<float *>(workspace), T, Ec, H, ld, x_dtype, st, SLICE);
+  if (rc > 0) return rc;
+  if (rc == 0) {
+    out->ld = ld;
+    return RF_OK;
+  }
+  LogitsArgs a{x, gate, shared_gate, reinterpret_cast<float *>(workspace), T, (int)H, (int)E, Ec};
+  switch (x_dtype) {
+    case RF_F32: launch_logits_tg<float>(a, p, gate_dtype, st); break;
+    case RF_F16: launch_logits_tg<__half>(a, p, gate_dtype, st); break;
+    default: launch_logits_tg<__nv_bfloat16>(a, p, gate_dtype, st); break;
+  }
+  out->ld = Ec;
+  return rf::check_launch((std::string(what) + "(logits)").c_str());
+}
+
+}  // namespace rf
+
 extern "C" size_t rf_moe_router_workspace_size(int64_t T, int64_t H, int64_t E, int has_shared_gate) {
   if (T <= 0 || H <= 0 || E <= 0) return 256;
   const int64_t Ec = E + (has_shared_gate ? 1 : 0);
@@ -444,43 +468,13 @@ extern "C" int rf_moe_router_topk(const void *x, int x_dtype, const void *gate, 
   b.round_dtype = round_dtype;
   b.entropy_k_min = entropy_k_min;
   if (gate) {
-    const Plan p = make_plan(T, (int)H, Ec);
-    const size_t need = (size_t)p.slices * (size_t)T * (size_t)Ec * sizeof(float);
-    RF_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0,
-                 "rf_moe_router_topk: workspace too small (see rf_moe_router_workspace_size)");
-    RF_CHECK_ARG(p.ttiles <= 0x7fffffff && p.slices <= 65535, "rf_moe_router_topk: too many tokens");
-    // Tensor cores when x and the gate share a 16-bit dtype and the shared
-    // gate (if any) is the row right after the gate's E rows: one tile per
-    // (128 tokens, slice of H), each slice a fixed MMA sequence, partials
-    // [slices][T][ld] summed in slice order by the top-k pass (the same bits
-    // whatever T is; few tokens still get one CTA per slice).  Otherwise the
-    // CUDA-core slices.
-    const size_t esz = (size_t)rf::dtype_size(gate_dtype);
-    const bool adjacent = !shared_gate ||
-                          (const char *)shared_gate == (const char *)gate + (size_t)E * (size_t)H * esz;
-    const int64_t ld = (Ec + 3) / 4 * 4;
-    int rc = -1;
-    if (x_dtype == gate_dtype && adjacent &&
-        workspace_bytes >= (size_t)p.slices * (size_t)T * (size_t)ld * sizeof(float))
-      rc = rf::tc_dense_f32(x, gate, reinterpret_cast<float *>(workspace), T, Ec, H, ld, x_dtype, st, SLICE);
-    if (rc > 0) return rc;
-    if (rc == 0) {
-      b.partial = reinterpret_cast<const float *>(workspace);
-      b.ksplit = p.slices;
-      b.ld = ld;
-    } else {
-      LogitsArgs a{x, gate, shared_gate, reinterpret_cast<float *>(workspace), T, (int)H, (int)E, Ec};
-      switch (x_dtype) {
-        case RF_F32: launch_logits_tg<float>(a, p, gate_dtype, st); break;
-        case RF_F16: launch_logits_tg<__half>(a, p, gate_dtype, st); break;
-        default: launch_logits_tg<__nv_bfloat16>(a, p, gate_dtype, st); break;
-      }
-      rc = rf::check_launch("rf_moe_router_topk(logits)");
-      if (rc) return rc;
-      b.partial = a.partial;
-      b.ksplit = p.slices;
-      b.ld = Ec;
-    }
+    rf::RouterLogits lg;
+    const int rc = rf::router_logits("rf_moe_router_topk", x, x_dtype, gate, gate_dtype, shared_gate, T, H, E,
+                                     workspace, workspace_bytes, st, &lg);
+    if (rc) return rc;
+    b.partial = lg.partial;
+    b.ksplit = lg.slices;
+    b.ld = lg.ld;
   }
   int64_t blocks = (T + TK_WARPS - 1) / TK_WARPS;
   const int64_t cap = (int64_t)rf::num_sms() * 8;

@@ -8,6 +8,7 @@ case raises :class:`reframework_b200._lib.RfMoeError`.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -32,6 +33,26 @@ def _require_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
         elif t.device != dev:
             raise _lib.RfMoeError(f"tensors on different devices: {dev} vs {t.device}")
     return dev
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device for a launch (nothing to do when it is)."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _f32_vector(t: Optional[torch.Tensor], n: int, dev: torch.device, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise _lib.RfMoeError(f"{what} must have {n} elements, got {tuple(t.shape)}")
+    if t.dtype == torch.float32 and t.device == dev and t.is_contiguous():
+        return t
+    return t.to(device=dev, dtype=torch.float32).contiguous()
+
+
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def rows_capacity(n_pairs: int, num_experts: int, align: int = ALIGN) -> int:
@@ -75,6 +96,61 @@ def router_topk(x: torch.Tensor, gate: Optional[torch.Tensor], top_k: int, *, re
         ptr(shared_gate), ptr(ss), ptr(w), ptr(i32), ptr(i64), ptr(lg), ptr(ws), ws_bytes,
         stream_of(dev))
     check(rc, "rf_moe_router_topk")
+    return w, i32, i64, lg, ss
+
+
+def router_grouped_topk(x: torch.Tensor, gate: Optional[torch.Tensor], top_k: int, *, scoring: str = "softmax",
+                        select_bias: Optional[torch.Tensor] = None, num_groups: int = 1, topk_groups: int = 1,
+                        group_score: str = "max", renormalize: bool = True, scale: float = 1.0,
+                        bias: Optional[torch.Tensor] = None, round_dtype: Optional[torch.dtype] = None,
+                        shared_gate: Optional[torch.Tensor] = None, want_logits: bool = False,
+                        ids64: bool = False, ids32: bool = True):
+    """Router logits, softmax or sigmoid scores, top-k by ``score + select_bias`` within the
+    ``topk_groups`` best of ``num_groups`` groups of consecutive experts; weights are the chosen
+    experts' scores, renormalised and times ``scale``.  ``gate=None``: ``x`` holds logits.
+
+    Returns what :func:`router_topk` returns: ``(weights fp32 [T,K], ids32 or None, ids64 or None,
+    logits or None, shared_scale or None)``.
+    """
+    dev = _require_cuda(x, gate, bias, select_bias, shared_gate)
+    if scoring not in _lib.SCORINGS:
+        raise ValueError(f"unknown scoring {scoring!r}; known: {tuple(_lib.SCORINGS)}")
+    if group_score not in _lib.GROUP_SCORES:
+        raise ValueError(f"unknown group score {group_score!r}; known: {tuple(_lib.GROUP_SCORES)}")
+    if x.dim() != 2:
+        raise _lib.RfMoeError(f"router_grouped_topk: x must be [T, H] (or [T, E] logits), got {tuple(x.shape)}")
+    x = _aligned16(x)
+    T, H = x.shape
+    E = H
+    if gate is not None:
+        if gate.dim() != 2 or gate.shape[1] != H:
+            raise _lib.RfMoeError(f"router_grouped_topk: gate must be [E, {H}], got {tuple(gate.shape)}")
+        gate = gate.contiguous()
+        E = gate.shape[0]
+    bias = _f32_vector(bias, E, dev, "router_grouped_topk: bias")
+    select_bias = _f32_vector(select_bias, E, dev, "router_grouped_topk: select_bias")
+    w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    i32 = torch.empty(T, top_k, dtype=torch.int32, device=dev) if ids32 else None
+    i64 = torch.empty(T, top_k, dtype=torch.int64, device=dev) if ids64 else None
+    lg = torch.empty(T, E, dtype=torch.float32, device=dev) if want_logits else None
+    ss = ws = None
+    ws_bytes = 0
+    if gate is not None:
+        if shared_gate is not None:
+            if shared_gate.numel() != H:
+                raise _lib.RfMoeError(f"router_grouped_topk: shared_gate must have {H} elements")
+            ss = torch.empty(T, dtype=torch.float32, device=dev)
+            shared_gate = shared_gate.to(dtype=gate.dtype).contiguous()
+        ws_bytes = int(lib().rf_moe_router_workspace_size(T, H, E, int(shared_gate is not None)))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib().rf_moe_router_grouped_topk(
+            ptr(x), dtype_code(x.dtype), ptr(gate), dtype_code(x.dtype if gate is None else gate.dtype), ptr(bias),
+            T, H, E, top_k, _lib.SCORINGS[scoring], ptr(select_bias), num_groups, topk_groups,
+            _lib.GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
+            -1 if round_dtype is None else dtype_code(round_dtype), ptr(shared_gate), ptr(ss), ptr(w), ptr(i32),
+            ptr(i64), ptr(lg), ptr(ws), ws_bytes, stream_of(dev))
+    check(rc, "rf_moe_router_grouped_topk")
     return w, i32, i64, lg, ss
 
 
@@ -350,3 +426,182 @@ def split_combine(y_hit: torch.Tensor, y_int8: torch.Tensor, row_of_slot: torch.
                                     stream_of(dev))
     check(rc, "rf_moe_split_combine")
     return out
+
+
+# ------------------------------------------------------------- 4-bit experts
+@dataclass
+class Int4Weights:
+    """Expert weights ``[S, N, K]`` as 4-bit codes with a 16-bit scale per ``group_size`` of K, in the
+    kernels' own layout (made by :func:`int4_pack` or :func:`int4_quantize`)."""
+
+    data: torch.Tensor     # uint8
+    scales: torch.Tensor   # layer dtype
+    slots: int             # S: experts
+    rows: int              # N (gated: 2I, gate rows then up rows)
+    cols: int              # K
+    group_size: int
+    gated: bool
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.scales.dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + 2 * self.scales.numel()
+
+    def to(self, device) -> "Int4Weights":
+        return Int4Weights(self.data.to(device), self.scales.to(device), self.slots, self.rows, self.cols,
+                           self.group_size, self.gated)
+
+
+def _int4_empty(slots: int, rows: int, cols: int, group_size: int, gated: bool, dtype: torch.dtype,
+                dev: torch.device, what: str) -> Int4Weights:
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.RfMoeError(f"{what}: 4-bit weights serve bfloat16 and float16 layers, got {dtype}")
+    args = (slots, rows, cols, group_size, int(gated))
+    nbytes = int(lib().rf_moe_int4_data_size(*args))
+    if nbytes < 0:
+        raise _lib.RfMoeError(f"{what}: {slots} weights of {rows} x {cols} with groups of {group_size} are not served "
+                              "(rows of each half and columns are multiples of 8, groups 32, 64 or 128)")
+    data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    scales = torch.empty(int(lib().rf_moe_int4_scales_count(*args)), dtype=dtype, device=dev)
+    return Int4Weights(data, scales, slots, rows, cols, group_size, gated)
+
+
+def int4_pack(codes: torch.Tensor, scales: torch.Tensor, *, group_size: int = 128, gated: bool = False) -> Int4Weights:
+    """Lays out ``weight[s, n, k] = scales[s, n, k // group_size] * (code[s, n, k] - 8)``.
+
+    ``codes`` [S, N, K/2] uint8, the even k in the low four bits of a byte; ``scales``
+    [S, N, ceil(K / group_size)] bfloat16 or float16.  ``gated``: the N rows are gate rows, then up rows (w1)."""
+    dev = _require_cuda(codes, scales)
+    if codes.dim() != 3 or codes.dtype != torch.uint8:
+        raise _lib.RfMoeError("int4_pack: codes must be uint8 [S, N, K/2]")
+    S, N, K = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
+    w = _int4_empty(S, N, K, group_size, gated, scales.dtype, dev, "int4_pack")
+    if tuple(scales.shape) != (S, N, -(-K // group_size)):
+        raise _lib.RfMoeError(f"int4_pack: scales must be {(S, N, -(-K // group_size))}, got {tuple(scales.shape)}")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    with _on(dev):
+        rc = lib().rf_moe_int4_pack(ptr(codes), ptr(scales), dtype_code(w.dtype), S, N, K, group_size, int(gated),
+                                    ptr(w.data), ptr(w.scales), stream_of(dev))
+    check(rc, "rf_moe_int4_pack")
+    return w
+
+
+def int4_quantize(weight: torch.Tensor, *, group_size: int = 128, gated: bool = False,
+                  dtype: Optional[torch.dtype] = None) -> Int4Weights:
+    """4-bit codes and scales of ``weight`` [S, N, K] (finite values, any float dtype).  A group's scale is its largest
+    magnitude / 7 rounded to five significant bits, so that every dequantised value is exact in the
+    layer dtype (``dtype``, default the weight's)."""
+    dev = _require_cuda(weight)
+    if weight.dim() != 3:
+        raise _lib.RfMoeError(f"int4_quantize: weight must be [S, N, K], got {tuple(weight.shape)}")
+    S, N, K = weight.shape
+    w = _int4_empty(S, N, K, group_size, gated, weight.dtype if dtype is None else dtype, dev, "int4_quantize")
+    weight = weight.detach().contiguous()
+    with _on(dev):
+        rc = lib().rf_moe_int4_quantize(ptr(weight), dtype_code(weight.dtype), dtype_code(w.dtype), S, N, K, group_size,
+                                        int(gated), ptr(w.data), ptr(w.scales), stream_of(dev))
+    check(rc, "rf_moe_int4_quantize")
+    return w
+
+
+def int4_dequantize(w: Int4Weights) -> torch.Tensor:
+    """``w`` as ``[S, N, K]`` in its layer dtype (each value rounded once; exact for :func:`int4_quantize`'s scales)."""
+    dev = _require_cuda(w.data, w.scales)
+    out = torch.empty(w.slots, w.rows, w.cols, dtype=w.dtype, device=dev)
+    with _on(dev):
+        rc = lib().rf_moe_int4_dequantize(ptr(w.data), ptr(w.scales), dtype_code(w.dtype), w.slots, w.rows, w.cols,
+                                          w.group_size, int(w.gated), ptr(out), stream_of(dev))
+    check(rc, "rf_moe_int4_dequantize")
+    return out
+
+
+def moe_experts_int4(x: torch.Tensor, w1: Int4Weights, w2: Int4Weights, weights: torch.Tensor, ids32: torch.Tensor, *,
+                     activation: str = "silu", shared_y: Optional[torch.Tensor] = None,
+                     shared_scale: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`moe_experts` with 4-bit weights (routing given): permute, gated products, down products and
+    an fp32 combine rounded once, ``out[t] = sum_k w[t,k] y + shared_scale * shared_y + residual``."""
+    dev = _require_cuda(x, w1.data, w2.data, weights, ids32, shared_y, shared_scale, residual, out)
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"unknown gated activation {activation!r}; known: {tuple(_lib.ACTIVATIONS)}")
+    dt = x.dtype
+    if x.dim() != 2 or ids32.dim() != 2 or weights.shape != ids32.shape or ids32.shape[0] != x.shape[0]:
+        raise _lib.RfMoeError("moe_experts_int4: need x [T, H], weights [T, K] and ids [T, K]")
+    T, H = x.shape
+    K, E, I = ids32.shape[1], w2.slots, w2.cols
+    if not w1.gated or w2.gated or w1.slots != E or w1.cols != H or w1.rows != 2 * I or w2.rows != H:
+        raise _lib.RfMoeError(f"moe_experts_int4: w1 must be a gated [E, 2I, {H}] and w2 an [E, {H}, I] weight, got "
+                              f"{(w1.slots, w1.rows, w1.cols)} and {(w2.slots, w2.rows, w2.cols)}")
+    if dt != w1.dtype or dt != w2.dtype:
+        raise _lib.RfMoeError(f"moe_experts_int4: x is {dt}, the weights serve {w1.dtype} and {w2.dtype}")
+    if ids32.dtype != torch.int32:
+        raise _lib.RfMoeError("moe_experts_int4: ids must be int32")
+    x, ids32 = _aligned16(x), ids32.contiguous()
+    if weights.dtype != torch.float32 or not weights.is_contiguous():
+        weights = weights.float().contiguous()
+    for name, t in (("shared_y", shared_y), ("residual", residual), ("out", out)):
+        if t is not None and (t.shape != x.shape or t.dtype != dt or not t.is_contiguous()):
+            raise _lib.RfMoeError(f"moe_experts_int4: {name} must be contiguous with x's shape and dtype")
+    shared_scale = _f32_vector(shared_scale, T, dev, "moe_experts_int4: shared_scale")
+    if out is None:
+        out = torch.empty(T, H, dtype=dt, device=dev)
+    L = lib()
+    ws_bytes = L.rf_moe_int4_experts_workspace_size(T, K, E, H, I)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = L.rf_moe_int4_experts(ptr(x), dtype_code(dt), ptr(w1.data), ptr(w1.scales), w1.group_size, ptr(w2.data),
+                                   ptr(w2.scales), w2.group_size, ptr(weights), ptr(ids32), T, K, E, H, I,
+                                   _lib.ACTIVATIONS[activation], ptr(shared_y), ptr(shared_scale), ptr(residual), ptr(out),
+                                   ptr(ws), ws_bytes, stream_of(dev))
+    check(rc, "rf_moe_int4_experts")
+    return out
+
+
+# ------------------------------------------- residual + RMSNorm, 8-bit output
+@dataclass
+class NormQ8:
+    q: Optional[torch.Tensor]          # [T, H] float8_e4m3fn
+    scales: Optional[torch.Tensor]     # [T, H / group_size] fp32 (one column for whole rows)
+    residual: torch.Tensor             # [T, H] the row that was normed (x itself without a residual)
+    normed: Optional[torch.Tensor]     # [T, H] in x's dtype
+
+
+def add_rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-6, group_size: int = 0,
+                   want_normed: bool = False, want_q: bool = True) -> NormQ8:
+    """``r = x + residual`` and its RMSNorm (reframework/layers/norm.py:27-53) as e4m3 values with an fp32 scale
+    per ``group_size`` columns (0: per row): the norm is ``q * scale``.  ``want_normed`` also returns it in x's dtype
+    (``want_q=False``: only that)."""
+    dev = _require_cuda(x, weight, residual, bias)
+    if x.dim() != 2:
+        raise _lib.RfMoeError(f"add_rmsnorm_q8: x must be [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    if group_size not in (0, 32, 64, 128) or (group_size and H % group_size):
+        raise _lib.RfMoeError("add_rmsnorm_q8: group_size must be 0 (the row), 32, 64 or 128 and divide H")
+    x = _aligned16(x)
+    r = x
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise _lib.RfMoeError("add_rmsnorm_q8: residual must have x's shape and dtype")
+        residual = _aligned16(residual)
+        r = torch.empty_like(x)
+    weight = _f32_vector(weight, H, dev, "add_rmsnorm_q8: weight")
+    bias = _f32_vector(bias, H, dev, "add_rmsnorm_q8: bias")
+    q = scales = None
+    if want_q:
+        q = torch.empty(T, H, dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty(T, H // group_size if group_size else 1, dtype=torch.float32, device=dev)
+    normed = torch.empty_like(x) if want_normed else None
+    with _on(dev):
+        rc = lib().rf_moe_add_rmsnorm_q8(ptr(x), ptr(residual), T, H, dtype_code(x.dtype), ptr(weight), ptr(bias),
+                                         float(eps), group_size, None if residual is None else ptr(r), ptr(normed),
+                                         ptr(q), ptr(scales), stream_of(dev))
+    check(rc, "rf_moe_add_rmsnorm_q8")
+    return NormQ8(q, scales, r, normed)

@@ -14,14 +14,14 @@ accumulates with a low-precision ``index_add_``).
 
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
 from .. import kernels as K
 from .._lib import RfMoeError
 
-__all__ = ["torch_fused_topk", "fused_experts"]
+__all__ = ["torch_fused_topk", "grouped_topk", "fused_experts", "fused_experts_int4"]
 
 
 def torch_fused_topk(gating_output: torch.Tensor, topk: int, renormalize: bool) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -32,6 +32,20 @@ def torch_fused_topk(gating_output: torch.Tensor, topk: int, renormalize: bool) 
         g = g.reshape(-1, g.shape[-1])
     w, _, ids, _, _ = K.router_topk(g.contiguous(), None, int(topk), renormalize=renormalize,
                                     ids64=True, ids32=False)
+    return w, ids
+
+
+def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool, num_groups: int = 1, topk_groups: int = 1,
+                 scoring: str = "softmax", select_bias: Optional[torch.Tensor] = None, group_score: str = "max",
+                 scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`torch_fused_topk` with softmax or sigmoid scores, a selection bias [E] and expert groups
+    (``kernels.router_grouped_topk``).  Returns (weights fp32 [M,K], ids int64 [M,K])."""
+    g = gating_output
+    if g.dim() != 2:
+        g = g.reshape(-1, g.shape[-1])
+    w, _, ids, _, _ = K.router_grouped_topk(g, None, int(topk), scoring=scoring, select_bias=select_bias,
+                                            num_groups=num_groups, topk_groups=topk_groups, group_score=group_score,
+                                            renormalize=renormalize, scale=scale, ids64=True, ids32=False)
     return w, ids
 
 
@@ -52,4 +66,16 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
     ids32 = topk_ids.to(torch.int32)
     w = topk_weights.float()
     out = K.moe_experts(xc.contiguous(), w1.contiguous(), w2.contiguous(), w, ids32, activation=activation)
+    return out if out.dtype == x.dtype else out.to(x.dtype)
+
+
+def fused_experts_int4(hidden_states: torch.Tensor, w1: K.Int4Weights, w2: K.Int4Weights, topk_weights: torch.Tensor,
+                       topk_ids: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """:func:`fused_experts` on 4-bit weights (``kernels.int4_quantize`` / ``int4_pack``; ``w1`` gated).  The
+    gated activation is rounded to the weights' 16-bit dtype, everything else is fp32 up to the output."""
+    if hidden_states.dim() != 2:
+        raise RfMoeError("fused_experts_int4: hidden_states must be [M, H]")
+    x = hidden_states
+    xc = x if x.dtype == w1.dtype else x.to(w1.dtype)
+    out = K.moe_experts_int4(xc, w1, w2, topk_weights, topk_ids.to(torch.int32), activation=activation)
     return out if out.dtype == x.dtype else out.to(x.dtype)

@@ -26,14 +26,21 @@ Opt-in extensions (default off, reference behaviour unchanged):
   ``num_shared_experts`` / ``shared_intermediate_size`` / ``shared_expert_gate``
   add always-on shared SwiGLU experts (optionally scaled by sigmoid(x.w_s));
   ``forward(x, residual=r)`` fuses ``+ r`` into the combine; ``device=``
-  allocates the parameters directly on a device.
+  allocates the parameters directly on a device;
+  ``set_routing(...)`` replaces softmax top-k by softmax or sigmoid scores with
+  a selection bias, expert groups and scaled weights;
+  ``quantize_experts(group_size)`` keeps the routed experts as 4-bit codes with
+  group scales; ``forward_add_residual_q8`` also hands the next layer its
+  normed input as e4m3 values with scales.
 """
 
 from __future__ import annotations
 
 import logging
+import math
 import time
 from collections import deque
+from dataclasses import dataclass
 from typing import Deque, Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -41,7 +48,7 @@ import torch.nn as nn
 
 from .. import env
 from .. import kernels as K
-from .._lib import ACTIVATIONS, RfMoeError
+from .._lib import ACTIVATIONS, GROUP_SCORES, SCORINGS, RfMoeError
 from .keys import expert_tensor
 from .offload_cache import ExpertOffloadCache, Prediction
 
@@ -118,6 +125,51 @@ def adjacent_router_weights(owner, gate: torch.Tensor,
     return cat[:-1], cat[-1]
 
 
+@dataclass(frozen=True)
+class Routing:
+    """The options of ``FusedMoE.set_routing`` (see ``kernels.router_grouped_topk``)."""
+
+    scoring: str = "softmax"
+    num_groups: int = 1
+    topk_groups: int = 1
+    group_score: str = "max"
+    scale: float = 1.0
+
+    def check(self, num_experts: int, top_k: int) -> None:
+        if self.scoring not in SCORINGS:
+            raise ValueError(f"unknown scoring {self.scoring!r}; known: {tuple(SCORINGS)}")
+        if self.group_score not in GROUP_SCORES:
+            raise ValueError(f"unknown group score {self.group_score!r}; known: {tuple(GROUP_SCORES)}")
+        if not 1 <= self.num_groups <= 32 or num_experts % self.num_groups:
+            raise ValueError(f"num_groups must be 1..32 and divide the {num_experts} experts, got {self.num_groups}")
+        if not 1 <= self.topk_groups <= self.num_groups:
+            raise ValueError(f"topk_groups must be 1..{self.num_groups}, got {self.topk_groups}")
+        per = num_experts // self.num_groups
+        if top_k > self.topk_groups * per:
+            raise ValueError(f"top_k = {top_k} experts do not fit into {self.topk_groups} groups of {per}")
+        if self.group_score == "top2" and self.num_groups > 1 and per < 2:
+            raise ValueError("a top-2 group score needs two experts in a group")
+        if not math.isfinite(self.scale):
+            raise ValueError(f"scale must be finite, got {self.scale}")
+
+
+def route_tokens(layer, x2: torch.Tensor, gate: torch.Tensor, shared_gate: Optional[torch.Tensor],
+                 round_dtype: Optional[torch.dtype], *, ids32: bool, ids64: bool):
+    """The layer's routing of ``x2`` (``kernels.router_topk``'s outputs), by its ``routing`` options if set."""
+    r = layer.routing
+    if r is None:
+        ek = layer.entropy_k_min if layer.entropy_adaptive_k else 0
+        return K.router_topk(x2, gate, layer.top_k, renormalize=layer.renormalize, bias=layer.router_bias,
+                             round_dtype=round_dtype, entropy_k_min=ek, shared_gate=shared_gate, ids32=ids32,
+                             ids64=ids64)
+    if layer.entropy_adaptive_k:
+        raise RfMoeError("the entropy-adaptive top-k is not available with set_routing()")
+    return K.router_grouped_topk(x2, gate, layer.top_k, scoring=r.scoring, select_bias=layer.select_bias,
+                                 num_groups=r.num_groups, topk_groups=r.topk_groups, group_score=r.group_score,
+                                 renormalize=layer.renormalize, scale=r.scale, bias=layer.router_bias,
+                                 round_dtype=round_dtype, shared_gate=shared_gate, ids32=ids32, ids64=ids64)
+
+
 def reference_output(out: torch.Tensor, x: torch.Tensor, hidden: int) -> torch.Tensor:
     """The layer output in the input's dtype and the reference's shape
     (moe_layer.py:519, ep.py:150): ``[x.shape[0], hidden]`` for an input of two
@@ -156,6 +208,9 @@ class FusedMoE(nn.Module):
         self.experts_w1 = nn.ParameterList([nn.Parameter(w1[e]) for e in range(E)])
         self.experts_w2 = nn.ParameterList([nn.Parameter(w2[e]) for e in range(E)])
         self.register_buffer("router_bias", None, persistent=False)
+        self.register_buffer("select_bias", None, persistent=False)
+        self.routing: Optional[Routing] = None
+        self._int4: Optional[Tuple[K.Int4Weights, K.Int4Weights]] = None
         self.num_shared_experts = num_shared_experts
         self.shared_intermediate_size = shared_intermediate_size
         if num_shared_experts:
@@ -195,11 +250,50 @@ class FusedMoE(nn.Module):
         """Add a fixed per-expert bias [E] to the router logits (None clears it)."""
         self.router_bias = None if bias is None else bias.detach().float().to(self.gate.device)
 
+    def set_routing(self, *, scoring: str = "softmax", select_bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+                    topk_groups: int = 1, group_score: str = "max", scale: float = 1.0) -> None:
+        """Route by softmax or sigmoid scores: the ``top_k`` largest ``score + select_bias`` among the
+        ``topk_groups`` best of ``num_groups`` groups of consecutive experts; the weights are the scores alone
+        (renormalised by the layer's ``renormalize``) times ``scale``.  ``select_bias`` [E] is a load-balancing
+        bias (-inf closes an expert)."""
+        r = Routing(scoring, int(num_groups), int(topk_groups), group_score, float(scale))
+        r.check(self.num_experts, self.top_k)
+        if select_bias is not None:
+            if select_bias.numel() != self.num_experts:
+                raise ValueError(f"select_bias must have {self.num_experts} elements, got {tuple(select_bias.shape)}")
+            select_bias = select_bias.detach().reshape(-1).float().to(self.gate.device)
+        self.routing, self.select_bias = r, select_bias
+
     # ------------------------------------------------------------ weight banks
     def _apply(self, fn, recurse=True):
         self._bank_cache = None
         self._router_cat = None
+        if self._int4 is not None:  # codes and scales change device with the layer, never their types
+            dev = fn(self._int4[0].data[:0]).device
+            self._int4 = (self._int4[0].to(dev), self._int4[1].to(dev))
         return super()._apply(fn, recurse)
+
+    def quantize_experts(self, group_size: int = 128) -> None:
+        """Keep the routed experts as 4-bit codes with one scale per ``group_size`` (32, 64 or 128) input
+        features (``kernels.int4_quantize``) and free their 16-bit weights.  The layer must be on its CUDA
+        device, resident (no offload cache) and of a 16-bit dtype; the router and the shared experts stay as they
+        are.  ``state_dict`` then returns the dequantised experts; ``load_state_dict`` comes before."""
+        if self.uses_offload:
+            raise RfMoeError("quantize_experts: the experts are offloaded; quantise a resident layer")
+        if self._int4 is not None:
+            raise RfMoeError("quantize_experts: the experts are quantised already")
+        w1b, w2b = self._resident_banks()
+        with torch.no_grad():
+            w1 = K.int4_quantize(w1b, group_size=group_size, gated=True)
+            w2 = K.int4_quantize(w2b, group_size=group_size)
+        self._int4 = (w1, w2)
+        self.experts_w1 = nn.ParameterList()
+        self.experts_w2 = nn.ParameterList()
+        self._bank_cache = None
+
+    @property
+    def uses_int4(self) -> bool:
+        return self._int4 is not None
 
     def invalidate_banks(self) -> None:
         """Call after replacing an expert parameter's ``.data`` directly."""
@@ -207,6 +301,8 @@ class FusedMoE(nn.Module):
         self._router_cat = None
 
     def _resident_banks(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        if self._int4 is not None:
+            raise RfMoeError("the experts are held as 4-bit codes (quantize_experts); there are no 16-bit banks")
         c = self._bank_cache
         if c is not None:
             return c
@@ -233,6 +329,8 @@ class FusedMoE(nn.Module):
     # ------------------------------------------------------------ offload setup
     def build_offload_cache(self, device: torch.device, lru_capacity: int) -> ExpertOffloadCache:
         """Stage the experts in a pinned host pool with ``lru_capacity`` device slots."""
+        if self._int4 is not None:
+            raise RfMoeError("build_offload_cache: the experts are held as 4-bit codes (quantize_experts)")
         self._cache = ExpertOffloadCache(device=torch.device(device), lru_capacity=lru_capacity,
                                          dtype=self.dtype)
         self._cache.load([{"w1": self.experts_w1[e], "w2": self.experts_w2[e]}
@@ -293,11 +391,8 @@ class FusedMoE(nn.Module):
         return adjacent_router_weights(self, self.gate, sg)
 
     def _router(self, x2: torch.Tensor, *, ids32: bool, ids64: bool):
-        ek = self.entropy_k_min if self.entropy_adaptive_k else 0
         gate, sg = self._router_weights()
-        return K.router_topk(x2, gate, self.top_k, renormalize=self.renormalize,
-                             bias=self.router_bias, round_dtype=self._round_dtype(), entropy_k_min=ek,
-                             shared_gate=sg, ids32=ids32, ids64=ids64)
+        return route_tokens(self, x2, gate, sg, self._round_dtype(), ids32=ids32, ids64=ids64)
 
     def _prep(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
@@ -332,6 +427,17 @@ class FusedMoE(nn.Module):
         spec = (norm.weight.detach(), None if bias is None else bias.detach(), float(norm.eps))
         res, normed = self._forward_impl(x, residual, spec)
         return self._shape_like(normed, x), self._shape_like(res, x)
+
+    def forward_add_residual_q8(self, x: torch.Tensor, residual: torch.Tensor, norm,
+                                group_size: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """:meth:`forward_add_residual` with the normed row in 8 bits for a following 8-bit product:
+        ``residual = moe(x) + residual``; ``norm(residual) = q * scales``.  Returns ``(q [M, H] float8_e4m3fn,
+        scales [M, H / group_size] fp32 (one column for ``group_size`` 0), residual)``."""
+        res, _ = self._forward_impl(x, residual, None)
+        bias = getattr(norm, "bias", None)
+        n = K.add_rmsnorm_q8(res, norm.weight.detach(), bias=None if bias is None else bias.detach(),
+                             eps=float(norm.eps), group_size=group_size)
+        return n.q, n.scales, self._shape_like(res, x)
 
     def _shape_like(self, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
         return reference_output(out, x, self.hidden_size)
@@ -369,6 +475,13 @@ class FusedMoE(nn.Module):
             out = self._forward_split(x2, w, ids32)
         elif self.uses_offload:
             out = self._forward_offload(x2, w, ids32, shared_y, sscale, res2, norm, normed)
+        elif self._int4 is not None:
+            if shared_done is not None:
+                torch.cuda.current_stream(x2.device).wait_event(shared_done)
+            out = K.moe_experts_int4(x2, *self._int4, w, ids32, activation=self.activation, shared_y=shared_y,
+                                     shared_scale=sscale, residual=res2)
+            if norm is not None:
+                normed = K.add_rmsnorm_q8(out, norm[0], bias=norm[1], eps=norm[2], want_q=False, want_normed=True).normed
         else:
             w1b, w2b = self._resident_banks()
             out = K.moe_experts(x2, w1b, w2b, w, ids32, activation=self.activation,
@@ -516,12 +629,17 @@ class FusedMoE(nn.Module):
         result = {} if result is None else result
         pre = f"{prefix}." if prefix else ""
         result[f"{pre}gate.weight"] = self.gate
+        if self.select_bias is not None:
+            result[f"{pre}gate.e_score_correction_bias"] = self.select_bias
         I = self.intermediate_size
-        for e in range(len(self.experts_w1)):
+        w1, w2 = self.experts_w1, self.experts_w2
+        if self._int4 is not None:
+            w1, w2 = (K.int4_dequantize(w) for w in self._int4)
+        for e in range(len(w1)):
             p = f"{pre}experts.{e}"
-            result[f"{p}.gate_proj.weight"] = self.experts_w1[e][:I]
-            result[f"{p}.up_proj.weight"] = self.experts_w1[e][I:]
-            result[f"{p}.down_proj.weight"] = self.experts_w2[e]
+            result[f"{p}.gate_proj.weight"] = w1[e][:I]
+            result[f"{p}.up_proj.weight"] = w1[e][I:]
+            result[f"{p}.down_proj.weight"] = w2[e]
         if self.num_shared_experts:
             Is = self.shared_intermediate_size
             for s in range(self.num_shared_experts):
@@ -538,10 +656,15 @@ class FusedMoE(nn.Module):
         Expert weights may also use the PhiMoE / Mixtral names ``w1`` / ``w3`` /
         ``w2`` (checkpoint/loader.py:83-103)."""
         pre = f"{prefix}." if prefix else ""
+        if self._int4 is not None and any(k.startswith(f"{pre}experts.") for k in state_dict):
+            raise RfMoeError("load_state_dict: the experts are held as 4-bit codes; load them before quantize_experts()")
         with torch.no_grad():
             g = f"{pre}gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
+            b = f"{pre}gate.e_score_correction_bias"
+            if b in state_dict and self.routing is not None:
+                self.select_bias = state_dict[b].detach().reshape(-1).float().to(self.gate.device)
             I = self.intermediate_size
             for e in range(len(self.experts_w1)):
                 p = f"{pre}experts.{e}"

@@ -44,7 +44,7 @@ from .. import kernels as K
 from .. import _lib as _lib_mod
 from .._lib import ACTIVATIONS, RfMoeError, check, dtype_code, lib, stream_of
 from ..moe.keys import expert_tensor
-from ..moe.moe_layer import FusedMoE, _bank_view, adjacent_router_weights, reference_output
+from ..moe.moe_layer import FusedMoE, _bank_view, adjacent_router_weights, reference_output, route_tokens
 from . import dist as _dist
 from .eplb import Placement, place_experts, split_rows
 
@@ -193,6 +193,8 @@ class EPFusedMoE(nn.Module):
         self.experts_w1 = nn.ParameterList([nn.Parameter(w1[j]) for j in range(n)])
         self.experts_w2 = nn.ParameterList([nn.Parameter(w2[j]) for j in range(n)])
         self.register_buffer("router_bias", None, persistent=False)
+        self.register_buffer("select_bias", None, persistent=False)
+        self.routing = None  # FusedMoE.set_routing's options, from the sharded layer
         self.entropy_adaptive_k = False
         self.entropy_k_min = 2
         self.precise_combine = False
@@ -247,6 +249,7 @@ class EPFusedMoE(nn.Module):
                 b1.copy_(w1b[ep.local_start:ep.local_end])
                 b2.copy_(w2b[ep.local_start:ep.local_end])
         ep.router_bias = base.router_bias
+        ep.routing, ep.select_bias = base.routing, base.select_bias
         ep.entropy_adaptive_k = base.entropy_adaptive_k
         ep.entropy_k_min = base.entropy_k_min
         ep.precise_combine = base.precise_combine
@@ -474,7 +477,6 @@ class EPFusedMoE(nn.Module):
         dev = x2.device
         T, H = x2.shape
         E, Kk, I = self.num_experts, self.top_k, self.intermediate_size
-        ek = self.entropy_k_min if self.entropy_adaptive_k else 0
         rdt = None if (self.router_dtype == torch.float32 or self.dtype == torch.float32) else self.dtype
         pg = self._pg()
         if self.trace is not None:
@@ -483,9 +485,7 @@ class EPFusedMoE(nn.Module):
         use_p2p = self.p2p and dev.type == "cuda"
         if T > 0:
             gate, sg = adjacent_router_weights(self, self.gate, self._shared_gate)
-            w, ids32, _, _, sscale = K.router_topk(x2, gate, Kk, renormalize=self.renormalize,
-                                                   bias=self.router_bias, round_dtype=rdt, entropy_k_min=ek,
-                                                   shared_gate=sg)
+            w, ids32, _, _, sscale = route_tokens(self, x2, gate, sg, rdt, ids32=True, ids64=False)
             # the peer push reads token rows through src_slot: no permuted copy
             p = K.permute(ids32, E, align=1, x=None if use_p2p else x2)
             counts = p.counts
@@ -805,6 +805,8 @@ class EPFusedMoE(nn.Module):
         result = {} if result is None else result
         pre = f"{prefix}." if prefix else ""
         result[f"{pre}gate.weight"] = self.gate
+        if self.select_bias is not None:
+            result[f"{pre}gate.e_score_correction_bias"] = self.select_bias
         I = self.intermediate_size
         for j, g in enumerate(range(self.local_start, self.local_end)):
             p = f"{pre}experts.{g}"
@@ -819,6 +821,9 @@ class EPFusedMoE(nn.Module):
             g = f"{pre}gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
+            b = f"{pre}gate.e_score_correction_bias"
+            if b in state_dict and self.routing is not None:
+                self.select_bias = state_dict[b].detach().reshape(-1).float().to(self.gate.device)
             I = self.intermediate_size
             for j, gg in enumerate(range(self.local_start, self.local_end)):
                 p = f"{pre}experts.{gg}"

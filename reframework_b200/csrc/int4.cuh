@@ -70,4 +70,19 @@ template <> __device__ __forceinline__ uint32_t int4_pair<__half>(uint32_t word,
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// One grouped product over all experts, rows in permuted order.
+struct Int4Gemm {
+  const void *a;                   // [rows, Kdim] in dtype
+  const uint8_t *w;
+  const void *scales;
+  void *out;                       // gated: [rows, N] in dtype; down: [rows, N] fp32
+  const int32_t *offsets, *counts; // [E+1], [E]
+  int64_t rows;
+  int E, Kdim, N;                  // N: output columns (I gated, H down)
+  int group, dtype, act;
+};
+
+// On CTA pairs (int4_pair.cu).
+int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st);
+
 }  // namespace rf

@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <string>
 
+#include "gemm.cuh"
 #include "int4.cuh"
 
 RF_DEVICE_ERROR_WORD();
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(SK_THREADS) int4_skinny_kernel(const SkinnyArg
 }
 
 template <typename T, int NT>
-int launch_skinny(const SkinnyArgs &p, bool gated, int max_active, cudaStream_t st) {
+int launch_skinny_t(const SkinnyArgs &p, bool gated, int max_active, cudaStream_t st) {
   const int units = (int)(gated ? p.sh.half_blocks : (p.sh.row_blocks() + 1) / 2);
   const dim3 grid(units, max_active);
   if (gated) {
@@ -234,6 +235,13 @@ int launch_skinny(const SkinnyArgs &p, bool gated, int max_active, cudaStream_t 
     else int4_skinny_kernel<T, NT, false, 1><<<grid, SK_THREADS, 0, st>>>(p);
   }
   return rf::check_launch(gated ? "4-bit gated products" : "4-bit down products");
+}
+
+int launch_skinny(const rf::Int4Gemm &g, bool gated, const int32_t *src, int topk, int max_active, cudaStream_t st) {
+  const SkinnyArgs p{g.a, g.w, g.scales, g.out, g.offsets, g.counts, src, topk, g.E, g.N, g.Kdim, g.group, g.act,
+                     rf::int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated)};
+  if (g.dtype == RF_F16) return launch_skinny_t<__half, 1>(p, gated, max_active, st);
+  return launch_skinny_t<__nv_bfloat16, 1>(p, gated, max_active, st);
 }
 
 // ------------------------------------------------------------------ combine
@@ -300,7 +308,7 @@ int launch_combine(const CombineArgs &a, cudaStream_t st) {
 
 // ------------------------------------------------------------------ workspace
 struct Layout {
-  size_t offsets, counts, row_of_slot, src, permute, permute_bytes, h, y, total;
+  size_t offsets, counts, row_of_slot, src, permute, permute_bytes, x, h, y, total;
   int64_t rows;
 };
 
@@ -321,6 +329,7 @@ Layout make_layout(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
   l.row_of_slot = take((size_t)l.rows * 4);
   l.src = take((size_t)l.rows * 4);
   l.permute = take(l.permute_bytes);
+  l.x = take((size_t)l.rows * (size_t)H * 2);
   l.h = take((size_t)l.rows * (size_t)I * 2);
   l.y = take((size_t)l.rows * (size_t)H * 4);
   l.total = at;
@@ -332,13 +341,15 @@ bool sizes_ok(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
          H < ((int64_t)1 << 28) && I < ((int64_t)1 << 28) && T <= 0x7fffffff / K;
 }
 
-template <typename T>
-int run_experts(SkinnyArgs &g, SkinnyArgs &d, const CombineArgs &cb, int max_active, cudaStream_t st) {
-  int rc = launch_skinny<T, 1>(g, true, max_active, st);
-  if (rc) return rc;
-  rc = launch_skinny<T, 1>(d, false, max_active, st);
-  if (rc) return rc;
-  return launch_combine<T>(cb, st);
+// The CTA-pair kernel from this many rows per expert on (the mean over the
+// experts that can have any: the counts are on the device).
+constexpr int64_t PAIR_ROWS = 8;
+
+bool use_pair(int64_t T, int64_t K, int64_t E) {
+  const int impl = rf::gemm_impl();
+  if (impl == 1) return false;
+  if (impl == 5) return true;
+  return T * K >= PAIR_ROWS * std::min(E, T * K);
 }
 
 }  // namespace
@@ -374,15 +385,19 @@ extern "C" int rf_moe_int4_experts(const void *x, int dtype, const void *w1, con
   int32_t *offsets = (int32_t *)(ws + l.offsets), *counts = (int32_t *)(ws + l.counts);
   int32_t *ros = (int32_t *)(ws + l.row_of_slot), *src = (int32_t *)(ws + l.src);
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = rf_moe_permute(topk_ids, T, K, E, 1, nullptr, 0, 0, offsets, counts, ros, src, nullptr, ws + l.permute,
-                          l.permute_bytes, stream);
+  const bool pair = use_pair(T, K, E);
+  int rc = rf_moe_permute(topk_ids, T, K, E, 1, pair ? x : nullptr, dtype, pair ? H : 0, offsets, counts, ros, src,
+                          pair ? ws + l.x : nullptr, ws + l.permute, l.permute_bytes, stream);
   if (rc) return rc;
-  SkinnyArgs g{x, (const uint8_t *)w1, w1_scales, ws + l.h, offsets, counts, src, (int)K, (int)E, (int)I, (int)H,
-               (int)w1_group, activation, rf::int4_shape(2 * I, H, w1_group, true)};
-  SkinnyArgs d{ws + l.h, (const uint8_t *)w2, w2_scales, ws + l.y, offsets, counts, nullptr, 1, (int)E, (int)H, (int)I,
-               (int)w2_group, activation, rf::int4_shape(H, I, w2_group, false)};
-  const CombineArgs cb{(const float *)(ws + l.y), ros, topk_weights, shared_y, shared_scale, residual, out, T, (int)K, (int)H};
+  const rf::Int4Gemm g{pair ? ws + l.x : x, (const uint8_t *)w1, w1_scales, ws + l.h, offsets, counts, l.rows, (int)E,
+                       (int)H, (int)I, (int)w1_group, dtype, activation};
+  const rf::Int4Gemm d{ws + l.h, (const uint8_t *)w2, w2_scales, ws + l.y, offsets, counts, l.rows, (int)E,
+                       (int)I, (int)H, (int)w2_group, dtype, activation};
   const int max_active = (int)std::min<int64_t>(E, T * K);
-  if (dtype == RF_F16) return run_experts<__half>(g, d, cb, max_active, st);
-  return run_experts<__nv_bfloat16>(g, d, cb, max_active, st);
+  rc = pair ? rf::launch_int4_pair(g, true, st) : launch_skinny(g, true, src, (int)K, max_active, st);
+  if (rc) return rc;
+  rc = pair ? rf::launch_int4_pair(d, false, st) : launch_skinny(d, false, nullptr, 1, max_active, st);
+  if (rc) return rc;
+  const CombineArgs cb{(const float *)(ws + l.y), ros, topk_weights, shared_y, shared_scale, residual, out, T, (int)K, (int)H};
+  return dtype == RF_F16 ? launch_combine<__half>(cb, st) : launch_combine<__nv_bfloat16>(cb, st);
 }

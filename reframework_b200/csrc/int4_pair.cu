@@ -1,0 +1,512 @@
+// Grouped products with 4-bit expert weights on CTA pairs (tcgen05.mma
+// cta_group::2), for experts with many rows.
+//
+//   gated: h[r, j] = act(a[r] . Wg[e, j]) * (a[r] . Wu[e, j])   stored in the layer dtype
+//   down:  y[r, n] = h[r] . W2[e, n]                            stored in fp32
+// As in gemm_pair.cu the weights are the MMA's M side (128 rows per CTA, 256
+// per pair) and the expert's token rows its N side (up to 256 in steps of 16,
+// half of them in each CTA's shared memory).  The weights arrive as 4-bit codes
+// (int4.cuh): eight warps read a CTA's codes straight from global memory into
+// registers, some stages ahead, turn each word into eight 16-bit values
+// scale * (code - 8) and write them where a TMA copy would have put 16-bit
+// weights (K-major, 128-byte swizzle).  The product of a code with a scale of
+// five significant bits is exact, so scales made by rf_moe_int4_quantize round
+// nothing here; a scale with more bits is rounded once per weight, to nearest.
+// Gated tiles put 16 gate rows and their 16 up rows into one quadrant of 32
+// TMEM lanes, so the epilogue pairs them with one shuffle.
+//
+// Roles (a cluster of two CTAs per pair, persistent, 14 warps):
+//   warp 0        TMA producer of this CTA's token rows
+//   warp 1        first CTA: MMA issuer
+//   warps 2-5     epilogue, one per TMEM lane quadrant
+//   warps 6-13    codes -> 16-bit rows, 16 rows each
+// A stage of the ring holds 128 k: it is full when the token bytes of both CTAs
+// and the arrivals of all sixteen code warps of the pair are in, and empty when
+// the MMAs that read it have committed.  Tiles (group, feature block, token
+// block; tokens fastest, so that running pairs share weights in L2) go to the
+// pairs round robin.  Every wait is bounded (2 s): on expiry the CTA sets the
+// device error word, both CTAs stop, let their copies land, drain their MMAs,
+// meet at a cluster barrier and free TMEM.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "int4.cuh"
+#include "gemm.cuh"
+
+RF_DEVICE_ERROR_WORD();
+#include "tc_pair_ptx.cuh"
+
+namespace {
+
+constexpr int Q_BK = 64;                        // swizzle atom depth (elements)
+constexpr int Q_KSUB = 2;                       // atoms per stage
+constexpr int Q_TOK = 256;                      // token rows per tile
+constexpr int Q_A_SUB = 128 * Q_BK * 2;         // 16 KB: this CTA's weight rows
+constexpr int Q_B_SUB = (Q_TOK / 2) * Q_BK * 2; // 16 KB: this CTA's token rows
+constexpr int Q_STAGES = 3;
+constexpr int Q_STAGE_BYTES = Q_KSUB * (Q_A_SUB + Q_B_SUB);
+constexpr int Q_EPI_WARPS = 4;
+constexpr int Q_CODE_WARPS = 8;
+constexpr int Q_THREADS = 32 * (2 + Q_EPI_WARPS + Q_CODE_WARPS);
+constexpr int Q_AHEAD = 4;                      // stages of codes in registers
+constexpr int Q_MAX_E = 1024;
+constexpr int Q_NUM_BARS = 2 * Q_STAGES + 5;    // full, empty, tmem full x2, tmem empty x2, drain
+constexpr int Q_N_BOXES = 5;                    // token boxes of 8, 16, 32, 64, 128 rows
+constexpr unsigned Q_EPI_SLEEP_NS = 256;
+constexpr uint64_t Q_ABORT_DRAIN_NS = 1000000;  // pause for copies in flight after an abort
+constexpr uint32_t Q_TMEM_COLS = 512;
+constexpr size_t Q_SMEM_BYTES =
+    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + Q_NUM_BARS * 8 + 16 + (size_t)(3 * Q_MAX_E + 1) * 4;
+static_assert(Q_SMEM_BYTES <= 227 * 1024, "shared memory");
+static_assert(Q_A_SUB % 1024 == 0 && Q_B_SUB % 1024 == 0, "swizzle atoms");
+
+struct PairArgs {
+  const int32_t *offsets, *counts;
+  const uint8_t *w;
+  const void *scales;
+  void *out;
+  int E, Kdim, N, n_fb;
+  int group, act;
+  rf::Int4Shape sh;
+};
+
+struct TokMaps {
+  CUtensorMap m[Q_N_BOXES];
+};
+
+__device__ __forceinline__ uint4 ldg_codes(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two 16-bit products, each rounded to nearest (exact for short scales).
+template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// SUBS: scale groups in a stage's 128 k (1, 2 or 4).
+template <typename T, bool GATED, int SUBS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
+    int4_pair_gemm(const __grid_constant__ TokMaps tmX, const PairArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sA = smem;
+  uint8_t *sB = sA + Q_STAGES * Q_KSUB * Q_A_SUB;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sB + Q_STAGES * Q_KSUB * Q_B_SUB);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Q_NUM_BARS);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+  int *tile_prefix = reinterpret_cast<int *>(tmem_holder + 4);  // [E+1]
+  int *g_row0 = tile_prefix + Q_MAX_E + 1;                        // [E]
+  int *g_cnt = g_row0 + Q_MAX_E;                                  // [E]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int E = p.E;
+  const int pair = (int)cluster_id_x(), npairs = (int)ncluster_x();
+  const uint32_t bar0 = smem_u32(bars);
+#define FULL(s) (bar0 + 8u * (uint32_t)(s))
+#define EMPTY(s) (bar0 + 8u * (uint32_t)(Q_STAGES + (s)))
+#define TFULL(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + (a)))
+#define TEMPTY(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 2 + (a)))
+  const uint32_t DRAIN = bar0 + 8u * (uint32_t)(2 * Q_STAGES + 4);
+  const uint32_t peer_abort = mapa_shared(smem_u32((const void *)abort_flag), rank ^ 1u);
+
+  // bounded wait with cluster-scope acquire; on expiry both CTAs are told to stop
+  auto pwait = [&](uint32_t bar, uint32_t parity, unsigned sleep_ns) -> bool {
+    if (mbar_try_cluster(bar, parity)) return true;
+    const uint64_t t0 = rf::globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+      if (sleep_ns) __nanosleep(sleep_ns);
+      if (mbar_try_cluster(bar, parity)) return true;
+      if ((it & 63) == 0) {
+        if (*abort_flag) return false;
+        if (rf::globaltimer_ns() - t0 > WAIT_LIMIT_NS) {
+          *abort_flag = 1;
+          st_cluster_u32(peer_abort, 1u);
+          rf_report(RF_DEV_WAIT_TIMEOUT);
+          return false;
+        }
+      }
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Q_STAGES; ++s) {
+      mbar_init(FULL(s), 1 + 2 * Q_CODE_WARPS);  // the first CTA's: its producer and the pair's code warps
+      mbar_init(EMPTY(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(TFULL(a), 1);
+      mbar_init(TEMPTY(a), 2 * Q_EPI_WARPS);
+    }
+    mbar_init(DRAIN, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 32)
+    for (int i = 0; i < Q_N_BOXES; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX.m[i]) : "memory");
+  for (int e = threadIdx.x; e < E; e += Q_THREADS) {
+    const int cnt = p.counts[e];
+    g_row0[e] = p.offsets[e];
+    g_cnt[e] = cnt;
+    tile_prefix[e + 1] = (cnt + Q_TOK - 1) / Q_TOK * p.n_fb;
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_holder), Q_TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  __syncthreads();
+  if (warp == 2) {  // inclusive scan of tile counts
+    int carry = 0;
+    for (int c = 0; c < E; c += 32) {
+      int v = c + lane < E ? tile_prefix[c + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (c + lane < E) tile_prefix[c + lane + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) tile_prefix[0] = 0;
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int total = tile_prefix[E];
+  const int num_kb = (p.Kdim + Q_BK * Q_KSUB - 1) / (Q_BK * Q_KSUB);  // stages per tile
+
+  // tile -> expert, first token row, token count, feature block
+  auto decode = [&](int t, int &e, int &row0, int &ntok, int &fb) {
+    int lo = 0, hi = E - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tile_prefix[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    const int cnt = g_cnt[lo];
+    const int ntb = (cnt + Q_TOK - 1) / Q_TOK;
+    const int local = t - tile_prefix[lo];
+    fb = local / ntb;
+    const int tb = local - fb * ntb;
+    e = lo;
+    row0 = g_row0[lo] + tb * Q_TOK;
+    ntok = min(Q_TOK, cnt - tb * Q_TOK);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------- token producer
+    if (lane == 0) {
+      const uint32_t full0 = mapa_shared(FULL(0), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += npairs) {
+        int e, row0, ntok, fb;
+        decode(t, e, row0, ntok, fb);
+        const int half = ((ntok + 15) & ~15) >> 1;  // token rows per CTA: a multiple of 8
+        int bi = 0;
+        while ((8 << bi) < half) ++bi;
+        const uint32_t bytes = (uint32_t)Q_KSUB * (uint32_t)(8 << bi) * (Q_BK * 2);  // per CTA
+        const int xrow = row0 + (rank ? half : 0);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pwait(EMPTY(stage), phase ^ 1u, 0)) {
+            ok = false;
+            break;
+          }
+          const uint32_t b_dst = smem_u32(sB + stage * Q_KSUB * Q_B_SUB);
+          if (rank == 0) mbar_expect_tx(FULL(stage), 2u * bytes);  // both CTAs load the same box sizes
+#pragma unroll
+          for (int j = 0; j < Q_KSUB; ++j)
+            tma_load_2d_pair(b_dst + (uint32_t)(j * Q_B_SUB), &tmX.m[bi], full0 + 8u * (uint32_t)stage,
+                             (kb * Q_KSUB + j) * Q_BK, xrow);
+          if (++stage == Q_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
+        const uint64_t t0 = rf::globaltimer_ns();
+        while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t IDESC = pair_idesc_base<T>();
+      const uint32_t peer_bars = mapa_shared(bar0, 1);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += npairs, ++it) {
+        int e, row0, ntok, fb;
+        decode(t, e, row0, ntok, fb);
+        const uint32_t idesc = IDESC | ((uint32_t)(((ntok + 15) & ~15) >> 3) << 17);
+        const int acc = it & 1;
+        if (!pwait(TEMPTY(acc), (uint32_t)(((it >> 1) & 1) ^ 1), 0)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pwait(FULL(stage), phase, 0)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * Q_KSUB * Q_A_SUB);
+          const uint32_t b0 = smem_u32(sB + stage * Q_KSUB * Q_B_SUB);
+#pragma unroll
+          for (int j = 0; j < Q_KSUB; ++j)
+#pragma unroll
+            for (int k = 0; k < Q_BK / 16; ++k)
+              tc_mma_pair(d, sw128_desc(a0 + j * Q_A_SUB + k * 32), sw128_desc(b0 + j * Q_B_SUB + k * 32), idesc,
+                          (kb | j | k) ? 1u : 0u);
+          tc_commit_pair(EMPTY(stage));  // frees the stage in both CTAs once read
+          tc_commit_pair(peer_bars + (EMPTY(stage) - bar0));
+          if (++stage == Q_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(TFULL(acc));
+        tc_commit_pair(peer_bars + (TFULL(acc) - bar0));
+      }
+      // no MMA may still be running when either CTA releases TMEM or exits
+      tc_commit_pair(DRAIN);
+      mbar_wait_teardown(DRAIN, 0);
+    }
+  } else if (warp < 2 + Q_EPI_WARPS) {
+    // ------------------------------------------------------------ epilogue
+    const int wq = warp & 3;  // the TMEM lane quadrant a warp can read
+    const uint32_t tempty0 = mapa_shared(TEMPTY(0), 0);
+    int it = 0;
+    for (int t = pair; t < total; t += npairs, ++it) {
+      int e, row0, ntok, fb;
+      decode(t, e, row0, ntok, fb);
+      const int acc = it & 1;
+      int ok = 1;
+      if (lane == 0) ok = pwait(TFULL(acc), (uint32_t)((it >> 1) & 1), Q_EPI_SLEEP_NS) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t tb = tmem_base + ((uint32_t)(wq * 32) << 16) + (uint32_t)(acc * 256);
+      const int np = (ntok + 15) & ~15;
+      // gated: lanes 0-15 of the quadrant hold gate rows, 16-31 the same features' up rows
+      const int f = GATED ? fb * 128 + (int)rank * 64 + wq * 16 + (lane & 15) : fb * 256 + (int)rank * 128 + wq * 32 + lane;
+      for (int c = 0; c < np; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(tb + (uint32_t)c, v);
+        tmem_ld_wait();
+        if (c + 16 >= np) {  // the accumulator is free for the pair's tile after next
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)acc);
+        }
+        if constexpr (GATED) {
+          const bool up = lane >= 16;
+          T *out = reinterpret_cast<T *>(p.out) + (int64_t)(row0 + c + (up ? 1 : 0)) * p.N + f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // tokens c + 2 i (lanes 0-15) and c + 2 i + 1
+            const uint32_t give = up ? v[2 * i] : v[2 * i + 1];
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 16);
+            const float g = __uint_as_float(up ? got : v[2 * i]);
+            const float u = __uint_as_float(up ? v[2 * i + 1] : got);
+            if (c + 2 * i + (up ? 1 : 0) < ntok && f < p.N)
+              out[(int64_t)(2 * i) * p.N] = rf::Cvt<T>::from_f(rf::act_gate(p.act, g) * u);
+          }
+        } else {
+          float *out = reinterpret_cast<float *>(p.out) + (int64_t)(row0 + c) * p.N + f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c + i < ntok && f < p.N) out[(int64_t)i * p.N] = __uint_as_float(v[i]);
+        }
+      }
+    }
+  } else {
+    // --------------------------------------------------------- code warps
+    const int j = warp - 2 - Q_EPI_WARPS;  // this warp's 16 of the CTA's 128 rows
+    const int g = lane >> 2, c = lane & 3;
+    const uint32_t full0 = mapa_shared(FULL(0), 0);
+    const int KB = (int)p.sh.k_blocks, groups = (int)p.sh.groups;
+    const int64_t row_blocks = p.sh.row_blocks();
+    // rows g and g + 8 of the 16, 16-byte pieces 4 h + c of their 128 bytes, swizzled
+    const uint32_t dst0 = (uint32_t)((j * 16 + g) * 128);
+    uint4 q[Q_AHEAD][Q_KSUB];
+    uint32_t sc[Q_AHEAD][SUBS];
+    // the read cursor: Q_AHEAD stages ahead of the written one
+    int rt = pair, rkb = 0;
+    const uint4 *rw = nullptr;
+    const uint32_t *rs = nullptr;
+    auto open_tile = [&]() {
+      if (rt >= total) return;
+      int e, row0, ntok, fb;
+      decode(rt, e, row0, ntok, fb);
+      // rows past the weight's own read its last block: never stored
+      int64_t rb;
+      if (GATED) rb = min((int64_t)fb * 8 + (int)rank * 4 + (j >> 1), p.sh.half_blocks - 1) + (j & 1 ? p.sh.half_blocks : 0);
+      else rb = min((int64_t)fb * 16 + (int)rank * 8 + j, row_blocks - 1);
+      rb += (int64_t)e * row_blocks;
+      rw = reinterpret_cast<const uint4 *>(p.w + rb * KB * rf::I4_BLOCK) + lane;
+      rs = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) + rb * groups * rf::I4_ROWS) + g;
+    };
+    auto read = [&](uint4 (&qs)[Q_KSUB], uint32_t (&ss)[SUBS]) {
+      if (rt >= total) return;
+#pragma unroll
+      for (int b = 0; b < Q_KSUB; ++b)  // k past the weight's own meets zero token values
+        qs[b] = ldg_codes(rw + (int64_t)min(rkb * Q_KSUB + b, KB - 1) * 32);
+#pragma unroll
+      for (int i = 0; i < SUBS; ++i) ss[i] = __ldg(rs + (int64_t)min(rkb * SUBS + i, groups - 1) * 8);
+      if (++rkb == num_kb) {
+        rkb = 0;
+        rt += npairs;
+        open_tile();
+      }
+    };
+    open_tile();
+#pragma unroll
+    for (int d = 0; d < Q_AHEAD; ++d) read(q[d], sc[d]);
+    int64_t left = 0;
+    for (int t = pair; t < total; t += npairs) left += num_kb;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+#pragma unroll
+      for (int d = 0; d < Q_AHEAD; ++d) {
+        if (left <= 0 || !ok) break;
+        int w = 1;
+        if (lane == 0) w = pwait(EMPTY(stage), phase ^ 1u, 0) ? 1 : 0;
+        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+        if (!ok) break;
+        const uint32_t a_dst = smem_u32(sA + stage * Q_KSUB * Q_A_SUB) + dst0;
+#pragma unroll
+        for (int b = 0; b < Q_KSUB; ++b) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // even rows write their halves in order, odd rows the second one
+            // first: eight neighbouring lanes then cover all 32 banks
+            const int h = i ^ (g & 1);
+            const uint32_t lo = h ? q[d][b].y : q[d][b].x, hi = h ? q[d][b].w : q[d][b].z;
+            // SUBS 4: a group is one half (32 k); 2: one block; 1: the stage
+            const uint32_t s = SUBS == 4 ? (h ? sc[d][(2 * b + 1) % SUBS] : sc[d][(2 * b) % SUBS]) : sc[d][b * SUBS / 2];
+            const uint32_t s_lo = __byte_perm(s, s, 0x1010), s_hi = __byte_perm(s, s, 0x3232);
+            const uint32_t at = a_dst + (uint32_t)(b * Q_A_SUB) + (uint32_t)((((4 * h + c) ^ g) & 7) * 16);
+            st_shared_v4(at, mul2<T>(rf::int4_pair<T>(lo, 0), s_lo), mul2<T>(rf::int4_pair<T>(lo, 1), s_lo),
+                         mul2<T>(rf::int4_pair<T>(lo, 2), s_lo), mul2<T>(rf::int4_pair<T>(lo, 3), s_lo));
+            st_shared_v4(at + 8 * 128, mul2<T>(rf::int4_pair<T>(hi, 0), s_hi), mul2<T>(rf::int4_pair<T>(hi, 1), s_hi),
+                         mul2<T>(rf::int4_pair<T>(hi, 2), s_hi), mul2<T>(rf::int4_pair<T>(hi, 3), s_hi));
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads through the async proxy
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(full0 + 8u * (uint32_t)stage);
+        read(q[d], sc[d]);
+        --left;
+        if (++stage == Q_STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  }
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA of the pair leaves while the other may still reach into it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, Q_TMEM_COLS);
+  }
+#undef FULL
+#undef EMPTY
+#undef TFULL
+#undef TEMPTY
+}
+
+template <typename T, bool GATED, int SUBS>
+int launch_pair_t(const TokMaps &mx, const PairArgs &p, cudaStream_t st) {
+  auto kern = int4_pair_gemm<T, GATED, SUBS>;
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  static int clusters = 0;
+  std::call_once(once, [&] {
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q_SMEM_BYTES);
+    if (err != cudaSuccess) return;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * std::max(1, rf::num_sms() / 2), 1, 1);
+    cfg.blockDim = dim3(Q_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Q_SMEM_BYTES;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    err = cudaOccupancyMaxActiveClusters(&clusters, (void *)kern, &cfg);
+  });
+  if (err != cudaSuccess || clusters < 1) {
+    cudaGetLastError();
+    return rf::fail(RF_ERR_CUDA, "4-bit products: the CTA-pair kernel does not fit this device");
+  }
+  kern<<<2 * clusters, Q_THREADS, Q_SMEM_BYTES, st>>>(mx, p);
+  return rf::check_launch(GATED ? "4-bit gated products (CTA pairs)" : "4-bit down products (CTA pairs)");
+}
+
+template <typename T, bool GATED>
+int launch_pair_g(const TokMaps &mx, const PairArgs &p, cudaStream_t st) {
+  if (p.group == 32) return launch_pair_t<T, GATED, 4>(mx, p, st);
+  if (p.group == 64) return launch_pair_t<T, GATED, 2>(mx, p, st);
+  return launch_pair_t<T, GATED, 1>(mx, p, st);
+}
+
+}  // namespace
+
+namespace rf {
+
+int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st) {
+  TokMaps mx;
+  const cuuint64_t dX[2] = {(cuuint64_t)g.Kdim, (cuuint64_t)g.rows};
+  const cuuint64_t sX[1] = {(cuuint64_t)g.Kdim * 2};
+  for (int i = 0; i < Q_N_BOXES; ++i) {
+    const cuuint32_t bX[2] = {Q_BK, (cuuint32_t)(8 << i)};
+    if (!tma_encode(&mx.m[i], g.dtype, 2, g.a, dX, sX, bX))
+      return rf::fail(RF_ERR_CUDA, "4-bit products: the token rows' tensor map could not be encoded");
+  }
+  PairArgs p;
+  p.offsets = g.offsets;
+  p.counts = g.counts;
+  p.w = g.w;
+  p.scales = g.scales;
+  p.out = g.out;
+  p.E = g.E;
+  p.Kdim = g.Kdim;
+  p.N = g.N;
+  p.n_fb = gated ? (g.N + 127) / 128 : (g.N + 255) / 256;
+  p.group = g.group;
+  p.act = g.act;
+  p.sh = int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated);
+  if (g.dtype == RF_F16) return gated ? launch_pair_g<__half, true>(mx, p, st) : launch_pair_g<__half, false>(mx, p, st);
+  return gated ? launch_pair_g<__nv_bfloat16, true>(mx, p, st) : launch_pair_g<__nv_bfloat16, false>(mx, p, st);
+}
+
+}  // namespace rf

@@ -15,6 +15,7 @@ DEV = torch.device("cuda")
 @pytest.fixture(autouse=True)
 def _device_clean(cuda_ok):
     yield
+    _lib.set_gemm_impl(0)
     assert _lib.device_status() == 0
 
 
@@ -90,7 +91,9 @@ def _check(x, q1, q2, w, ids, g1, g2, activation="silu", **kw):
 
 @pytest.mark.parametrize("T,E,top_k,H,I,g1,g2", CASES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_experts(T, E, top_k, H, I, g1, g2, dtype):
+@pytest.mark.parametrize("impl", [0, 1, 5])  # automatic, few-row kernel, CTA pairs
+def test_experts(T, E, top_k, H, I, g1, g2, dtype, impl):
+    _lib.set_gemm_impl(impl)
     _check(*_case(T, E, top_k, H, I, g1, g2, dtype, T + I), g1, g2)
 
 
@@ -114,8 +117,10 @@ def test_shared_output_and_residual(T, gated_scale):
 
 
 @pytest.mark.parametrize("T", [2, 40, 600])
-def test_uneven_routing(T):
+@pytest.mark.parametrize("impl", [1, 5])
+def test_uneven_routing(T, impl):
     """All tokens on one expert, the same expert twice in a token, and experts without tokens."""
+    _lib.set_gemm_impl(impl)
     x, q1, q2, w, ids = _case(T, 16, 2, 128, 96, 64, 64, torch.bfloat16, 21)
     ids[:] = 5
     _check(x, q1, q2, w, ids, 64, 64)
@@ -148,7 +153,9 @@ def test_empty_batch_strided_and_unaligned_inputs():
 
 
 @pytest.mark.parametrize("T", [4, 300])
-def test_not_a_number_stays_in_its_token(T):
+@pytest.mark.parametrize("impl", [1, 5])
+def test_not_a_number_stays_in_its_token(T, impl):
+    _lib.set_gemm_impl(impl)
     x, q1, q2, w, ids = _case(T, 4, 2, 128, 64, 64, 64, torch.bfloat16, 24)
     w1, w2 = K.int4_pack(*q1, group_size=64, gated=True), K.int4_pack(*q2, group_size=64)
     want = K.moe_experts_int4(x, w1, w2, w, ids)
@@ -204,9 +211,11 @@ def test_against_16_bit_experts():
 
 
 @pytest.mark.parametrize("T", [1, 64, 400])
-def test_scales_with_all_their_bits(T):
+@pytest.mark.parametrize("impl", [1, 5])
+def test_scales_with_all_their_bits(T, impl):
     """Checkpoint scales: where scale * (code - 8) needs more than 16 bits holds, the operand may be rounded once
     (half a step, u = eps / 2 of each weight): both products' bounds grow by u of their magnitudes."""
+    _lib.set_gemm_impl(impl)
     g1 = g2 = 64
     x, q1, q2, w, ids = _case(T, 4, 2, 256, 128, g1, g2, torch.bfloat16, 29, fine=True)
     w1, w2 = K.int4_pack(*q1, group_size=g1, gated=True), K.int4_pack(*q2, group_size=g2)

@@ -6,8 +6,8 @@
 // As in gemm_pair.cu the weights are the MMA's M side (128 rows per CTA, 256
 // per pair) and the expert's token rows its N side (up to 256 in steps of 16,
 // half of them in each CTA's shared memory).  The weights arrive as 4-bit codes
-// (int4.cuh): eight warps read a CTA's codes straight from global memory into
-// registers, some stages ahead, turn each word into eight 16-bit values
+// (int4.cuh): bulk copies bring a CTA's codes and scales into a ring of their
+// own, and code warps turn each word into eight 16-bit values
 // scale * (code - 8) and write them where a TMA copy would have put 16-bit
 // weights (K-major, 128-byte swizzle).  The product of a code with a scale of
 // five significant bits is exact, so scales made by rf_moe_int4_quantize round
@@ -19,9 +19,11 @@
 //   warp 0        TMA producer of this CTA's token rows
 //   warp 1        first CTA: MMA issuer
 //   warps 2-5     epilogue, one per TMEM lane quadrant
-//   warps 6-13    codes -> 16-bit rows, 16 rows each
+//   warps 6-17    codes -> 16-bit rows: four warps (32 rows each) for each of
+//                 the ring's three slots, so that three stages are in work at
+//                 a time; each warp copies its own codes, one use ahead
 // A stage of the ring holds 128 k: it is full when the token bytes of both CTAs
-// and the arrivals of all sixteen code warps of the pair are in, and empty when
+// and the arrivals of the pair's eight code warps of its slot are in, and empty when
 // the MMAs that read it have committed.  Tiles (group, feature block, token
 // block; tokens fastest, so that running pairs share weights in L2) go to the
 // pairs round robin.  Every wait is bounded (2 s): on expiry the CTA sets the
@@ -50,18 +52,20 @@ constexpr int Q_B_SUB = (Q_TOK / 2) * Q_BK * 2; // 16 KB: this CTA's token rows
 constexpr int Q_STAGES = 3;
 constexpr int Q_STAGE_BYTES = Q_KSUB * (Q_A_SUB + Q_B_SUB);
 constexpr int Q_EPI_WARPS = 4;
-constexpr int Q_CODE_WARPS = 8;
-constexpr int Q_THREADS = 32 * (2 + Q_EPI_WARPS + Q_CODE_WARPS);
-constexpr int Q_AHEAD = 4;                      // stages of codes in registers
+constexpr int Q_CODE_WARPS = 4;                 // code warps of a stage: 32 weight rows each
+constexpr int Q_THREADS = 32 * (2 + Q_EPI_WARPS + Q_STAGES * Q_CODE_WARPS);
+constexpr int Q_CODE_BYTES = Q_KSUB * rf::I4_BLOCK + 128;  // 16 rows x 128 k and up to four groups' scales
 constexpr int Q_MAX_E = 1024;
-constexpr int Q_NUM_BARS = 2 * Q_STAGES + 5;    // full, empty, tmem full x2, tmem empty x2, drain
+constexpr int Q_NUM_BARS = 2 * Q_STAGES + 5 + Q_CODE_WARPS * Q_STAGES;  // full, empty, tmem full x2, tmem empty x2, drain, codes
 constexpr int Q_N_BOXES = 5;                    // token boxes of 8, 16, 32, 64, 128 rows
 constexpr unsigned Q_EPI_SLEEP_NS = 256;
 constexpr uint64_t Q_ABORT_DRAIN_NS = 1000000;  // pause for copies in flight after an abort
 constexpr uint32_t Q_TMEM_COLS = 512;
 constexpr size_t Q_SMEM_BYTES =
-    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + Q_NUM_BARS * 8 + 16 + (size_t)(3 * Q_MAX_E + 1) * 4;
+    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + (size_t)Q_CODE_WARPS * Q_STAGES * 2 * Q_CODE_BYTES + Q_NUM_BARS * 8 + 16 +
+    (size_t)(Q_MAX_E + 1) * 4;
 static_assert(Q_SMEM_BYTES <= 227 * 1024, "shared memory");
+static_assert(Q_CODE_BYTES % 16 == 0, "bulk copies");
 static_assert(Q_A_SUB % 1024 == 0 && Q_B_SUB % 1024 == 0, "swizzle atoms");
 
 struct PairArgs {
@@ -78,11 +82,20 @@ struct TokMaps {
   CUtensorMap m[Q_N_BOXES];
 };
 
-__device__ __forceinline__ uint4 ldg_codes(const uint4 *p) {
+// Bulk copy of `bytes` (a multiple of 16) to this CTA's shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
@@ -109,12 +122,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sA = smem;
   uint8_t *sB = sA + Q_STAGES * Q_KSUB * Q_A_SUB;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sB + Q_STAGES * Q_KSUB * Q_B_SUB);
+  uint8_t *sQ = sB + Q_STAGES * Q_KSUB * Q_B_SUB;  // [code warp][two row blocks] codes, then scales
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sQ + Q_CODE_WARPS * Q_STAGES * 2 * Q_CODE_BYTES);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Q_NUM_BARS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   int *tile_prefix = reinterpret_cast<int *>(tmem_holder + 4);  // [E+1]
-  int *g_row0 = tile_prefix + Q_MAX_E + 1;                        // [E]
-  int *g_cnt = g_row0 + Q_MAX_E;                                  // [E]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -126,6 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 #define TFULL(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + (a)))
 #define TEMPTY(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 2 + (a)))
   const uint32_t DRAIN = bar0 + 8u * (uint32_t)(2 * Q_STAGES + 4);
+#define CODES(i) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 5 + (i)))
   const uint32_t peer_abort = mapa_shared(smem_u32((const void *)abort_flag), rank ^ 1u);
 
   // bounded wait with cluster-scope acquire; on expiry both CTAs are told to stop
@@ -157,17 +170,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
       mbar_init(TEMPTY(a), 2 * Q_EPI_WARPS);
     }
     mbar_init(DRAIN, 1);
+    for (int i = 0; i < Q_CODE_WARPS * Q_STAGES; ++i) mbar_init(CODES(i), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x == 32)
     for (int i = 0; i < Q_N_BOXES; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX.m[i]) : "memory");
-  for (int e = threadIdx.x; e < E; e += Q_THREADS) {
-    const int cnt = p.counts[e];
-    g_row0[e] = p.offsets[e];
-    g_cnt[e] = cnt;
-    tile_prefix[e + 1] = (cnt + Q_TOK - 1) / Q_TOK * p.n_fb;
-  }
+  for (int e = threadIdx.x; e < E; e += Q_THREADS) tile_prefix[e + 1] = (p.counts[e] + Q_TOK - 1) / Q_TOK * p.n_fb;
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_holder), Q_TMEM_COLS);
     tmem_relinquish_pair();
@@ -202,13 +211,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
       if (tile_prefix[mid] <= t) lo = mid;
       else hi = mid - 1;
     }
-    const int cnt = g_cnt[lo];
+    const int cnt = __ldg(p.counts + lo);
     const int ntb = (cnt + Q_TOK - 1) / Q_TOK;
     const int local = t - tile_prefix[lo];
     fb = local / ntb;
     const int tb = local - fb * ntb;
     e = lo;
-    row0 = g_row0[lo] + tb * Q_TOK;
+    row0 = __ldg(p.offsets + lo) + tb * Q_TOK;
     ntok = min(Q_TOK, cnt - tb * Q_TOK);
   };
 
@@ -343,61 +352,81 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     }
   } else {
     // --------------------------------------------------------- code warps
-    const int j = warp - 2 - Q_EPI_WARPS;  // this warp's 16 of the CTA's 128 rows
+    // Warp cw serves one slot of the ring, so it follows every phase of the
+    // barriers that it waits for: stages s = slot, slot + Q_STAGES, ...
+    const int cw = warp - 2 - Q_EPI_WARPS;
+    const int slot = cw / Q_CODE_WARPS, j = cw % Q_CODE_WARPS;  // its 32 of the CTA's 128 rows: blocks 2 j, 2 j + 1
     const int g = lane >> 2, c = lane & 3;
-    const uint32_t full0 = mapa_shared(FULL(0), 0);
+    const uint32_t full = mapa_shared(FULL(slot), 0);
     const int KB = (int)p.sh.k_blocks, groups = (int)p.sh.groups;
-    const int64_t row_blocks = p.sh.row_blocks();
-    // rows g and g + 8 of the 16, 16-byte pieces 4 h + c of their 128 bytes, swizzled
-    const uint32_t dst0 = (uint32_t)((j * 16 + g) * 128);
-    uint4 q[Q_AHEAD][Q_KSUB];
-    uint32_t sc[Q_AHEAD][SUBS];
-    // the read cursor: Q_AHEAD stages ahead of the written one
-    int rt = pair, rkb = 0;
-    const uint4 *rw = nullptr;
-    const uint32_t *rs = nullptr;
-    auto open_tile = [&]() {
-      if (rt >= total) return;
+    const uint32_t codes = smem_u32(sQ) + (uint32_t)(cw * 2 * Q_CODE_BYTES);
+    const int steps = pair < total ? ((total - 1 - pair) / npairs + 1) * num_kb : 0;
+    int t = pair, kb = slot;  // of the next stage to copy
+    const uint8_t *rw[2];
+    const uint8_t *rs[2];
+    auto open_tile = [&]() {  // the tile of stage kb >= num_kb or the first one
+      while (kb >= num_kb) {
+        kb -= num_kb;
+        t += npairs;
+      }
+      if (t >= total) return;
       int e, row0, ntok, fb;
-      decode(rt, e, row0, ntok, fb);
-      // rows past the weight's own read its last block: never stored
-      int64_t rb;
-      if (GATED) rb = min((int64_t)fb * 8 + (int)rank * 4 + (j >> 1), p.sh.half_blocks - 1) + (j & 1 ? p.sh.half_blocks : 0);
-      else rb = min((int64_t)fb * 16 + (int)rank * 8 + j, row_blocks - 1);
-      rb += (int64_t)e * row_blocks;
-      rw = reinterpret_cast<const uint4 *>(p.w + rb * KB * rf::I4_BLOCK) + lane;
-      rs = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) + rb * groups * rf::I4_ROWS) + g;
+      decode(t, e, row0, ntok, fb);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        // rows past the weight's own read its last block: never stored
+        int64_t rb;
+        if (GATED) rb = min((int64_t)fb * 8 + (int)rank * 4 + j, p.sh.half_blocks - 1) + (r ? p.sh.half_blocks : 0);
+        else rb = min((int64_t)fb * 16 + (int)rank * 8 + 2 * j + r, p.sh.half_blocks - 1);
+        rb += (int64_t)e * p.sh.row_blocks();
+        rw[r] = p.w + rb * KB * rf::I4_BLOCK;
+        rs[r] = reinterpret_cast<const uint8_t *>(p.scales) + rb * groups * (rf::I4_ROWS * 2);
+      }
     };
-    auto read = [&](uint4 (&qs)[Q_KSUB], uint32_t (&ss)[SUBS]) {
-      if (rt >= total) return;
+    // k blocks and groups past the weight's own are not copied: the token
+    // values they meet are zero, and what the slot holds there is finite
+    auto copy = [&]() {
+      const uint32_t nb = (uint32_t)min(Q_KSUB, KB - kb * Q_KSUB) * rf::I4_BLOCK;
+      const uint32_t ns = (uint32_t)min(SUBS, groups - kb * SUBS) * (rf::I4_ROWS * 2);
+      mbar_expect_tx(CODES(cw), 2 * (nb + ns));
 #pragma unroll
-      for (int b = 0; b < Q_KSUB; ++b)  // k past the weight's own meets zero token values
-        qs[b] = ldg_codes(rw + (int64_t)min(rkb * Q_KSUB + b, KB - 1) * 32);
-#pragma unroll
-      for (int i = 0; i < SUBS; ++i) ss[i] = __ldg(rs + (int64_t)min(rkb * SUBS + i, groups - 1) * 8);
-      if (++rkb == num_kb) {
-        rkb = 0;
-        rt += npairs;
-        open_tile();
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t dst = codes + (uint32_t)(r * Q_CODE_BYTES);
+        bulk_load(dst, rw[r] + (int64_t)kb * (Q_KSUB * rf::I4_BLOCK), nb, CODES(cw));
+        bulk_load(dst + Q_KSUB * rf::I4_BLOCK, rs[r] + (int64_t)kb * (SUBS * rf::I4_ROWS * 2), ns, CODES(cw));
       }
     };
     open_tile();
-#pragma unroll
-    for (int d = 0; d < Q_AHEAD; ++d) read(q[d], sc[d]);
-    int64_t left = 0;
-    for (int t = pair; t < total; t += npairs) left += num_kb;
-    int stage = 0;
+    if (lane == 0 && slot < steps) copy();
+    // rows g and g + 8 of a block, 16-byte pieces 4 h + c of their 128 bytes, swizzled
+    const uint32_t a_dst = smem_u32(sA + slot * Q_KSUB * Q_A_SUB) + (uint32_t)((j * 32 + g) * 128);
     uint32_t phase = 0;
     bool ok = true;
-    while (left > 0 && ok) {
+    for (int s = slot; s < steps; s += Q_STAGES, phase ^= 1u) {
+      ok = __all_sync(0xffffffffu, pwait(CODES(cw), phase, 0));  // the warp leaves together
+      if (!ok) break;
+      uint4 q[2][Q_KSUB];
+      uint32_t sc[2][SUBS];
+      const int last = groups - 1 - kb * SUBS;
 #pragma unroll
-      for (int d = 0; d < Q_AHEAD; ++d) {
-        if (left <= 0 || !ok) break;
-        int w = 1;
-        if (lane == 0) w = pwait(EMPTY(stage), phase ^ 1u, 0) ? 1 : 0;
-        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-        if (!ok) break;
-        const uint32_t a_dst = smem_u32(sA + stage * Q_KSUB * Q_A_SUB) + dst0;
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t src = codes + (uint32_t)(r * Q_CODE_BYTES);
+#pragma unroll
+        for (int b = 0; b < Q_KSUB; ++b) q[r][b] = ld_shared_v4(src + (uint32_t)(b * rf::I4_BLOCK + lane * 16));
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i)
+          sc[r][i] = ld_shared_u32(src + (uint32_t)(Q_KSUB * rf::I4_BLOCK + min(i, last) * (rf::I4_ROWS * 2) + g * 4));
+      }
+      // the codes are in registers: the slot's next ones may come
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      kb += Q_STAGES;
+      if (kb >= num_kb) open_tile();
+      if (lane == 0 && s + Q_STAGES < steps) copy();
+      ok = __all_sync(0xffffffffu, pwait(EMPTY(slot), phase ^ 1u, 0));
+      if (!ok) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
 #pragma unroll
         for (int b = 0; b < Q_KSUB; ++b) {
 #pragma unroll
@@ -405,27 +434,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
             // even rows write their halves in order, odd rows the second one
             // first: eight neighbouring lanes then cover all 32 banks
             const int h = i ^ (g & 1);
-            const uint32_t lo = h ? q[d][b].y : q[d][b].x, hi = h ? q[d][b].w : q[d][b].z;
+            const uint32_t lo = h ? q[r][b].y : q[r][b].x, hi = h ? q[r][b].w : q[r][b].z;
             // SUBS 4: a group is one half (32 k); 2: one block; 1: the stage
-            const uint32_t s = SUBS == 4 ? (h ? sc[d][(2 * b + 1) % SUBS] : sc[d][(2 * b) % SUBS]) : sc[d][b * SUBS / 2];
-            const uint32_t s_lo = __byte_perm(s, s, 0x1010), s_hi = __byte_perm(s, s, 0x3232);
-            const uint32_t at = a_dst + (uint32_t)(b * Q_A_SUB) + (uint32_t)((((4 * h + c) ^ g) & 7) * 16);
+            const uint32_t sv = SUBS == 4 ? (h ? sc[r][(2 * b + 1) % SUBS] : sc[r][(2 * b) % SUBS]) : sc[r][b * SUBS / 2];
+            const uint32_t s_lo = __byte_perm(sv, sv, 0x1010), s_hi = __byte_perm(sv, sv, 0x3232);
+            const uint32_t at = a_dst + (uint32_t)(b * Q_A_SUB + r * 16 * 128) + (uint32_t)((((4 * h + c) ^ g) & 7) * 16);
             st_shared_v4(at, mul2<T>(rf::int4_pair<T>(lo, 0), s_lo), mul2<T>(rf::int4_pair<T>(lo, 1), s_lo),
                          mul2<T>(rf::int4_pair<T>(lo, 2), s_lo), mul2<T>(rf::int4_pair<T>(lo, 3), s_lo));
             st_shared_v4(at + 8 * 128, mul2<T>(rf::int4_pair<T>(hi, 0), s_hi), mul2<T>(rf::int4_pair<T>(hi, 1), s_hi),
                          mul2<T>(rf::int4_pair<T>(hi, 2), s_hi), mul2<T>(rf::int4_pair<T>(hi, 3), s_hi));
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads through the async proxy
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(full0 + 8u * (uint32_t)stage);
-        read(q[d], sc[d]);
-        --left;
-        if (++stage == Q_STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(full);
+    }
+    if (!ok && lane == 0) {  // copies in flight land before this CTA can exit (bounded pause)
+      const uint64_t t0 = rf::globaltimer_ns();
+      while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -436,6 +463,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, Q_TMEM_COLS);
   }
+#undef CODES
 #undef FULL
 #undef EMPTY
 #undef TFULL

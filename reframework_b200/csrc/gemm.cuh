@@ -60,6 +60,9 @@ int launch_simt_grouped_gemm(const GroupedGemmArgs &g, bool gated, cudaStream_t 
 // A 16-bit tiled tensor map with the 128-byte swizzle (gemm_tc.cu).
 bool tma_encode(CUtensorMap *m, int dtype, int rank, const void *base, const cuuint64_t *dims,
                 const cuuint64_t *strides, const cuuint32_t *box);
+// A tiled map of a 2-D tensor without a swizzle: rows of `cols` elements, `row_bytes` apart.
+bool tma_encode_plain(CUtensorMap *m, CUtensorMapDataType type, const void *base, uint64_t cols, uint64_t rows,
+                      uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows);
 // The GEMM implementation chosen by rf_moe_set_gemm_impl (0 = automatic).
 int gemm_impl();
 

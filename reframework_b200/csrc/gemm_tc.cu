@@ -771,6 +771,16 @@ bool tma_encode(CUtensorMap *m, int dtype, int rank, const void *base, const cuu
                 const cuuint64_t *strides, const cuuint32_t *box) {
   return encode(m, dtype, rank, base, dims, strides, box);
 }
+bool tma_encode_plain(CUtensorMap *m, CUtensorMapDataType type, const void *base, uint64_t cols, uint64_t rows,
+                      uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  return fn(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 int gemm_impl() { return g_gemm_impl; }
 
 // out[m, n] = sum_k a[m, k] * w[n, k] for m < M, n < N, fp32 accumulation

@@ -53,25 +53,26 @@ constexpr int Q_STAGES = 3;
 constexpr int Q_STAGE_BYTES = Q_KSUB * (Q_A_SUB + Q_B_SUB);
 constexpr int Q_EPI_WARPS = 4;
 constexpr int Q_CODE_WARPS = 4;                 // code warps of a stage: 32 weight rows each
-constexpr int Q_THREADS = 32 * (2 + Q_EPI_WARPS + Q_STAGES * Q_CODE_WARPS);
-constexpr int Q_CODE_BYTES = Q_KSUB * rf::I4_BLOCK + 128;  // 16 rows x 128 k and up to four groups' scales
+constexpr int Q_COPY_WARP = 2 + Q_EPI_WARPS + Q_STAGES * Q_CODE_WARPS;  // the last warp
+constexpr int Q_THREADS = 32 * (Q_COPY_WARP + 1);
+constexpr int Q_BLOCKS = 8;                     // row blocks (16 rows) of a CTA's stage
+constexpr int Q_CODE_BYTES = Q_BLOCKS * Q_KSUB * rf::I4_BLOCK;  // 8 KB
+constexpr int Q_SCALE_BYTES = Q_BLOCKS * 4 * rf::I4_ROWS * 2;   // 1 KB: up to four groups
 constexpr int Q_MAX_E = 1024;
-constexpr int Q_NUM_BARS = 2 * Q_STAGES + 5 + Q_CODE_WARPS * Q_STAGES;  // full, empty, tmem full x2, tmem empty x2, drain, codes
+constexpr int Q_NUM_BARS = 4 * Q_STAGES + 5;  // full, empty, tmem full x2, tmem empty x2, drain, codes full, codes empty
 constexpr int Q_N_BOXES = 5;                    // token boxes of 8, 16, 32, 64, 128 rows
 constexpr unsigned Q_EPI_SLEEP_NS = 256;
 constexpr uint64_t Q_ABORT_DRAIN_NS = 1000000;  // pause for copies in flight after an abort
 constexpr uint32_t Q_TMEM_COLS = 512;
 constexpr size_t Q_SMEM_BYTES =
-    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + (size_t)Q_CODE_WARPS * Q_STAGES * 2 * Q_CODE_BYTES + Q_NUM_BARS * 8 + 16 +
+    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + (size_t)Q_STAGES * (Q_CODE_BYTES + Q_SCALE_BYTES) + Q_NUM_BARS * 8 + 16 +
     (size_t)(Q_MAX_E + 1) * 4;
 static_assert(Q_SMEM_BYTES <= 227 * 1024, "shared memory");
-static_assert(Q_CODE_BYTES % 16 == 0, "bulk copies");
+static_assert(Q_CODE_BYTES % 128 == 0 && Q_SCALE_BYTES % 128 == 0, "TMA destinations");
 static_assert(Q_A_SUB % 1024 == 0 && Q_B_SUB % 1024 == 0, "swizzle atoms");
 
 struct PairArgs {
   const int32_t *offsets, *counts;
-  const uint8_t *w;
-  const void *scales;
   void *out;
   int E, Kdim, N, n_fb;
   int group, act;
@@ -82,11 +83,14 @@ struct TokMaps {
   CUtensorMap m[Q_N_BOXES];
 };
 
-// Bulk copy of `bytes` (a multiple of 16) to this CTA's shared memory, counted on `bar`.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
-               : "memory");
+// Arrive on either CTA's barrier with a release of CTA scope.  What it hands
+// over stays on this SM: rows in this CTA's shared memory that this SM's tensor
+// core reads (ordered by the proxy fence before it), or this CTA's TMEM; only
+// the count is kept by the other CTA.  A release of cluster scope here waited
+// 1000-1800 cycles, once per stage (measured with clock64 on C2's shapes: the
+// stage period fell from 1760 cycles with it).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
@@ -117,13 +121,14 @@ template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_
 // SUBS: scale groups in a stage's 128 k (1, 2 or 4).
 template <typename T, bool GATED, int SUBS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
-    int4_pair_gemm(const __grid_constant__ TokMaps tmX, const PairArgs p) {
+    int4_pair_gemm(const __grid_constant__ TokMaps tmX, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmS, const PairArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sA = smem;
   uint8_t *sB = sA + Q_STAGES * Q_KSUB * Q_A_SUB;
-  uint8_t *sQ = sB + Q_STAGES * Q_KSUB * Q_B_SUB;  // [code warp][two row blocks] codes, then scales
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sQ + Q_CODE_WARPS * Q_STAGES * 2 * Q_CODE_BYTES);
+  uint8_t *sQ = sB + Q_STAGES * Q_KSUB * Q_B_SUB;  // [slot] codes, then scales
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sQ + Q_STAGES * (Q_CODE_BYTES + Q_SCALE_BYTES));
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Q_NUM_BARS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   int *tile_prefix = reinterpret_cast<int *>(tmem_holder + 4);  // [E+1]
@@ -138,7 +143,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 #define TFULL(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + (a)))
 #define TEMPTY(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 2 + (a)))
   const uint32_t DRAIN = bar0 + 8u * (uint32_t)(2 * Q_STAGES + 4);
-#define CODES(i) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 5 + (i)))
+#define CFULL(s) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 5 + (s)))
+#define CEMPTY(s) (bar0 + 8u * (uint32_t)(3 * Q_STAGES + 5 + (s)))
   const uint32_t peer_abort = mapa_shared(smem_u32((const void *)abort_flag), rank ^ 1u);
 
   // bounded wait with cluster-scope acquire; on expiry both CTAs are told to stop
@@ -162,17 +168,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Q_STAGES; ++s) {
-      mbar_init(FULL(s), 1 + 2 * Q_CODE_WARPS);  // the first CTA's: its producer and the pair's code warps
+      mbar_init(FULL(s), 1 + 2 * Q_CODE_WARPS);  // the first CTA's: its token producer and the pair's code warps
       mbar_init(EMPTY(s), 1);
+      mbar_init(CFULL(s), 1);
+      mbar_init(CEMPTY(s), Q_CODE_WARPS);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(TFULL(a), 1);
       mbar_init(TEMPTY(a), 2 * Q_EPI_WARPS);
     }
     mbar_init(DRAIN, 1);
-    for (int i = 0; i < Q_CODE_WARPS * Q_STAGES; ++i) mbar_init(CODES(i), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 32 * Q_COPY_WARP) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmW) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmS) : "memory");
   }
   if (threadIdx.x == 32)
     for (int i = 0; i < Q_N_BOXES; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX.m[i]) : "memory");
@@ -328,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         if (c + 16 >= np) {  // the accumulator is free for the pair's tile after next
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)acc);
+          if (lane == 0) mbar_arrive_remote(tempty0 + 8u * (uint32_t)acc);
         }
         if constexpr (GATED) {
           const bool up = lane >= 16;
@@ -350,81 +361,81 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         }
       }
     }
+  } else if (warp == Q_COPY_WARP) {
+    // ---------------------------------------------- codes and scales producer
+    if (lane == 0) {
+      const int64_t row_blocks = p.sh.row_blocks();
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += npairs) {
+        int e, row0, ntok, fb;
+        decode(t, e, row0, ntok, fb);
+        // two boxes of four row blocks: gate and up, or eight in a row; blocks
+        // past the weight's own are some other rows or zeros, never stored
+        const int rb0 = (int)((int64_t)e * row_blocks) + (GATED ? fb * 8 + (int)rank * 4 : fb * 16 + (int)rank * 8);
+        const int rb1 = rb0 + (GATED ? (int)p.sh.half_blocks : 4);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pwait(CEMPTY(stage), phase ^ 1u, 0)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = smem_u32(sQ) + (uint32_t)(stage * (Q_CODE_BYTES + Q_SCALE_BYTES));
+          const uint32_t sdst = dst + Q_CODE_BYTES;
+          mbar_expect_tx(CFULL(stage), Q_CODE_BYTES + Q_BLOCKS * SUBS * rf::I4_ROWS * 2);
+          tma_load_2d(dst, &tmW, CFULL(stage), kb * (Q_KSUB * rf::I4_BLOCK / 4), rb0);
+          tma_load_2d(dst + Q_CODE_BYTES / 2, &tmW, CFULL(stage), kb * (Q_KSUB * rf::I4_BLOCK / 4), rb1);
+          tma_load_2d(sdst, &tmS, CFULL(stage), kb * (SUBS * rf::I4_ROWS), rb0);
+          tma_load_2d(sdst + Q_SCALE_BYTES / 2, &tmS, CFULL(stage), kb * (SUBS * rf::I4_ROWS), rb1);
+          if (++stage == Q_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
+        const uint64_t t0 = rf::globaltimer_ns();
+        while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
+      }
+    }
   } else {
     // --------------------------------------------------------- code warps
-    // Warp cw serves one slot of the ring, so it follows every phase of the
+    // Warp cw serves one slot of the rings, so it follows every phase of the
     // barriers that it waits for: stages s = slot, slot + Q_STAGES, ...
     const int cw = warp - 2 - Q_EPI_WARPS;
-    const int slot = cw / Q_CODE_WARPS, j = cw % Q_CODE_WARPS;  // its 32 of the CTA's 128 rows: blocks 2 j, 2 j + 1
+    const int slot = cw / Q_CODE_WARPS, j = cw % Q_CODE_WARPS;  // its 32 of the CTA's 128 rows
     const int g = lane >> 2, c = lane & 3;
-    const uint32_t full = mapa_shared(FULL(slot), 0);
-    const int KB = (int)p.sh.k_blocks, groups = (int)p.sh.groups;
-    const uint32_t codes = smem_u32(sQ) + (uint32_t)(cw * 2 * Q_CODE_BYTES);
+    const uint32_t codes = smem_u32(sQ) + (uint32_t)(slot * (Q_CODE_BYTES + Q_SCALE_BYTES));
     const int steps = pair < total ? ((total - 1 - pair) / npairs + 1) * num_kb : 0;
-    int t = pair, kb = slot;  // of the next stage to copy
-    const uint8_t *rw[2];
-    const uint8_t *rs[2];
-    auto open_tile = [&]() {  // the tile of stage kb >= num_kb or the first one
-      while (kb >= num_kb) {
-        kb -= num_kb;
-        t += npairs;
-      }
-      if (t >= total) return;
-      int e, row0, ntok, fb;
-      decode(t, e, row0, ntok, fb);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        // rows past the weight's own read its last block: never stored
-        int64_t rb;
-        if (GATED) rb = min((int64_t)fb * 8 + (int)rank * 4 + j, p.sh.half_blocks - 1) + (r ? p.sh.half_blocks : 0);
-        else rb = min((int64_t)fb * 16 + (int)rank * 8 + 2 * j + r, p.sh.half_blocks - 1);
-        rb += (int64_t)e * p.sh.row_blocks();
-        rw[r] = p.w + rb * KB * rf::I4_BLOCK;
-        rs[r] = reinterpret_cast<const uint8_t *>(p.scales) + rb * groups * (rf::I4_ROWS * 2);
-      }
-    };
-    // k blocks and groups past the weight's own are not copied: the token
-    // values they meet are zero, and what the slot holds there is finite
-    auto copy = [&]() {
-      const uint32_t nb = (uint32_t)min(Q_KSUB, KB - kb * Q_KSUB) * rf::I4_BLOCK;
-      const uint32_t ns = (uint32_t)min(SUBS, groups - kb * SUBS) * (rf::I4_ROWS * 2);
-      mbar_expect_tx(CODES(cw), 2 * (nb + ns));
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t dst = codes + (uint32_t)(r * Q_CODE_BYTES);
-        bulk_load(dst, rw[r] + (int64_t)kb * (Q_KSUB * rf::I4_BLOCK), nb, CODES(cw));
-        bulk_load(dst + Q_KSUB * rf::I4_BLOCK, rs[r] + (int64_t)kb * (SUBS * rf::I4_ROWS * 2), ns, CODES(cw));
-      }
-    };
-    open_tile();
-    if (lane == 0 && slot < steps) copy();
-    // rows g and g + 8 of a block, 16-byte pieces 4 h + c of their 128 bytes, swizzled
+    // rows g and g + 8 of a block, 16-byte pieces 4 h + c of their 128 bytes,
+    // swizzled; the first one written has h = g & 1
+    const uint32_t piece0 = (uint32_t)((((4 * (g & 1) + c) ^ g) & 7) * 16), piece1 = piece0 ^ 64u;
     const uint32_t a_dst = smem_u32(sA + slot * Q_KSUB * Q_A_SUB) + (uint32_t)((j * 32 + g) * 128);
+    const uint32_t full = mapa_shared(FULL(slot), 0);
     uint32_t phase = 0;
-    bool ok = true;
     for (int s = slot; s < steps; s += Q_STAGES, phase ^= 1u) {
-      ok = __all_sync(0xffffffffu, pwait(CODES(cw), phase, 0));  // the warp leaves together
+      bool ok = __all_sync(0xffffffffu, pwait(CFULL(slot), phase, 0));  // the warp leaves together
       if (!ok) break;
       uint4 q[2][Q_KSUB];
       uint32_t sc[2][SUBS];
-      const int last = groups - 1 - kb * SUBS;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t src = codes + (uint32_t)(r * Q_CODE_BYTES);
+        // the tile's rows 32 j .. 32 j + 15 and the next 16: a gate block and
+        // its up block, or two neighbours
+        const int at = GATED ? 4 * r + j : 2 * j + r;
+        const uint32_t src = codes + (uint32_t)(at * Q_KSUB * rf::I4_BLOCK + lane * 16);
+        const uint32_t ss = codes + Q_CODE_BYTES +
+                            (uint32_t)((at >> 2) * (Q_SCALE_BYTES / 2) + (at & 3) * (SUBS * rf::I4_ROWS * 2) + g * 4);
 #pragma unroll
-        for (int b = 0; b < Q_KSUB; ++b) q[r][b] = ld_shared_v4(src + (uint32_t)(b * rf::I4_BLOCK + lane * 16));
+        for (int b = 0; b < Q_KSUB; ++b) q[r][b] = ld_shared_v4(src + (uint32_t)(b * rf::I4_BLOCK));
 #pragma unroll
-        for (int i = 0; i < SUBS; ++i)
-          sc[r][i] = ld_shared_u32(src + (uint32_t)(Q_KSUB * rf::I4_BLOCK + min(i, last) * (rf::I4_ROWS * 2) + g * 4));
+        for (int i = 0; i < SUBS; ++i) sc[r][i] = ld_shared_u32(ss + (uint32_t)(i * rf::I4_ROWS * 2));
       }
-      // the codes are in registers: the slot's next ones may come
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      kb += Q_STAGES;
-      if (kb >= num_kb) open_tile();
-      if (lane == 0 && s + Q_STAGES < steps) copy();
-      ok = __all_sync(0xffffffffu, pwait(EMPTY(slot), phase ^ 1u, 0));
-      if (!ok) break;
+      if (lane == 0) mbar_arrive(CEMPTY(slot));  // the codes are in registers
+      // 16-bit values of rows g (v[..][0]) and g + 8, before the wait: only
+      // the stores stay between a slot's release and its next use
+      uint32_t v[2][Q_KSUB][2][2][4];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -438,21 +449,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
             // SUBS 4: a group is one half (32 k); 2: one block; 1: the stage
             const uint32_t sv = SUBS == 4 ? (h ? sc[r][(2 * b + 1) % SUBS] : sc[r][(2 * b) % SUBS]) : sc[r][b * SUBS / 2];
             const uint32_t s_lo = __byte_perm(sv, sv, 0x1010), s_hi = __byte_perm(sv, sv, 0x3232);
-            const uint32_t at = a_dst + (uint32_t)(b * Q_A_SUB + r * 16 * 128) + (uint32_t)((((4 * h + c) ^ g) & 7) * 16);
-            st_shared_v4(at, mul2<T>(rf::int4_pair<T>(lo, 0), s_lo), mul2<T>(rf::int4_pair<T>(lo, 1), s_lo),
-                         mul2<T>(rf::int4_pair<T>(lo, 2), s_lo), mul2<T>(rf::int4_pair<T>(lo, 3), s_lo));
-            st_shared_v4(at + 8 * 128, mul2<T>(rf::int4_pair<T>(hi, 0), s_hi), mul2<T>(rf::int4_pair<T>(hi, 1), s_hi),
-                         mul2<T>(rf::int4_pair<T>(hi, 2), s_hi), mul2<T>(rf::int4_pair<T>(hi, 3), s_hi));
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              v[r][b][i][0][m] = mul2<T>(rf::int4_pair<T>(lo, m), s_lo);
+              v[r][b][i][1][m] = mul2<T>(rf::int4_pair<T>(hi, m), s_hi);
+              asm volatile("" : "+r"(v[r][b][i][0][m]), "+r"(v[r][b][i][1][m]));  // computed here
+            }
           }
         }
       }
+      ok = __all_sync(0xffffffffu, pwait(EMPTY(slot), phase ^ 1u, 0));
+      if (!ok) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int b = 0; b < Q_KSUB; ++b)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t at = a_dst + (uint32_t)(b * Q_A_SUB + r * 16 * 128) + (i ? piece1 : piece0);
+            const uint32_t(&w)[2][4] = v[r][b][i];
+            st_shared_v4(at, w[0][0], w[0][1], w[0][2], w[0][3]);
+            st_shared_v4(at + 8 * 128, w[1][0], w[1][1], w[1][2], w[1][3]);
+          }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads through the async proxy
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(full);
-    }
-    if (!ok && lane == 0) {  // copies in flight land before this CTA can exit (bounded pause)
-      const uint64_t t0 = rf::globaltimer_ns();
-      while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
+      if (lane == 0) mbar_arrive_remote(full);
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -463,7 +484,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, Q_TMEM_COLS);
   }
-#undef CODES
+#undef CFULL
+#undef CEMPTY
 #undef FULL
 #undef EMPTY
 #undef TFULL
@@ -471,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 }
 
 template <typename T, bool GATED, int SUBS>
-int launch_pair_t(const TokMaps &mx, const PairArgs &p, cudaStream_t st) {
+int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
   auto kern = int4_pair_gemm<T, GATED, SUBS>;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
@@ -496,15 +518,15 @@ int launch_pair_t(const TokMaps &mx, const PairArgs &p, cudaStream_t st) {
     cudaGetLastError();
     return rf::fail(RF_ERR_CUDA, "4-bit products: the CTA-pair kernel does not fit this device");
   }
-  kern<<<2 * clusters, Q_THREADS, Q_SMEM_BYTES, st>>>(mx, p);
+  kern<<<2 * clusters, Q_THREADS, Q_SMEM_BYTES, st>>>(mx, mw, ms, p);
   return rf::check_launch(GATED ? "4-bit gated products (CTA pairs)" : "4-bit down products (CTA pairs)");
 }
 
 template <typename T, bool GATED>
-int launch_pair_g(const TokMaps &mx, const PairArgs &p, cudaStream_t st) {
-  if (p.group == 32) return launch_pair_t<T, GATED, 4>(mx, p, st);
-  if (p.group == 64) return launch_pair_t<T, GATED, 2>(mx, p, st);
-  return launch_pair_t<T, GATED, 1>(mx, p, st);
+int launch_pair_g(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
+  if (p.group == 32) return launch_pair_t<T, GATED, 4>(mx, mw, ms, p, st);
+  if (p.group == 64) return launch_pair_t<T, GATED, 2>(mx, mw, ms, p, st);
+  return launch_pair_t<T, GATED, 1>(mx, mw, ms, p, st);
 }
 
 }  // namespace
@@ -523,8 +545,6 @@ int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st) {
   PairArgs p;
   p.offsets = g.offsets;
   p.counts = g.counts;
-  p.w = g.w;
-  p.scales = g.scales;
   p.out = g.out;
   p.E = g.E;
   p.Kdim = g.Kdim;
@@ -533,8 +553,19 @@ int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st) {
   p.group = g.group;
   p.act = g.act;
   p.sh = int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated);
-  if (g.dtype == RF_F16) return gated ? launch_pair_g<__half, true>(mx, p, st) : launch_pair_g<__half, false>(mx, p, st);
-  return gated ? launch_pair_g<__nv_bfloat16, true>(mx, p, st) : launch_pair_g<__nv_bfloat16, false>(mx, p, st);
+  // codes as [E * row blocks][k blocks * 128] words, scales as [E * row blocks][groups * 16]
+  const uint64_t rows = (uint64_t)g.E * (uint64_t)p.sh.row_blocks();
+  const uint32_t scale_cols = (uint32_t)(Q_KSUB * Q_BK / g.group * rf::I4_ROWS);
+  CUtensorMap mw, ms;
+  if (!tma_encode_plain(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, g.w, (uint64_t)p.sh.k_blocks * (I4_BLOCK / 4), rows,
+                        (uint64_t)p.sh.k_blocks * I4_BLOCK, Q_KSUB * I4_BLOCK / 4, 4) ||
+      !tma_encode_plain(&ms, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.scales, (uint64_t)p.sh.groups * I4_ROWS, rows,
+                        (uint64_t)p.sh.groups * I4_ROWS * 2, scale_cols, 4))
+    return rf::fail(RF_ERR_CUDA, "4-bit products: the weights' tensor maps could not be encoded");
+  if (g.dtype == RF_F16)
+    return gated ? launch_pair_g<__half, true>(mx, mw, ms, p, st) : launch_pair_g<__half, false>(mx, mw, ms, p, st);
+  return gated ? launch_pair_g<__nv_bfloat16, true>(mx, mw, ms, p, st)
+               : launch_pair_g<__nv_bfloat16, false>(mx, mw, ms, p, st);
 }
 
 }  // namespace rf

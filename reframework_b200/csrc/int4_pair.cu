@@ -118,6 +118,21 @@ template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_
   return *reinterpret_cast<const uint32_t *>(&r);
 }
 
+// 16 token columns of a quadrant: lanes 0-15 hold gate sums, lanes 16-31 the up
+// sums of the same 16 features.  Lanes 0-15 finish the even tokens, 16-31 the
+// odd ones (out and left are for this lane's first).
+template <typename T, int ACT>
+__device__ __forceinline__ void store_gated(const uint32_t (&v)[16], int lane, T *out, int N, int left) {
+  const bool up = lane >= 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i, out += 2 * (int64_t)N) {
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? v[2 * i] : v[2 * i + 1], 16);
+    const float g = __uint_as_float(up ? got : v[2 * i]);
+    const float u = __uint_as_float(up ? v[2 * i + 1] : got);
+    if (2 * i < left) *out = rf::Cvt<T>::from_f(rf::act_gate_t<ACT>(g) * u);
+  }
+}
+
 // SUBS: scale groups in a stage's 128 k (1, 2 or 4).
 template <typename T, bool GATED, int SUBS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
@@ -342,22 +357,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
           if (lane == 0) mbar_arrive_remote(tempty0 + 8u * (uint32_t)acc);
         }
         if constexpr (GATED) {
-          const bool up = lane >= 16;
-          T *out = reinterpret_cast<T *>(p.out) + (int64_t)(row0 + c + (up ? 1 : 0)) * p.N + f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // tokens c + 2 i (lanes 0-15) and c + 2 i + 1
-            const uint32_t give = up ? v[2 * i] : v[2 * i + 1];
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 16);
-            const float g = __uint_as_float(up ? got : v[2 * i]);
-            const float u = __uint_as_float(up ? v[2 * i + 1] : got);
-            if (c + 2 * i + (up ? 1 : 0) < ntok && f < p.N)
-              out[(int64_t)(2 * i) * p.N] = rf::Cvt<T>::from_f(rf::act_gate(p.act, g) * u);
-          }
+          T *out = reinterpret_cast<T *>(p.out) + (int64_t)(row0 + c + (lane >> 4)) * p.N + f;
+          const int left = f < p.N ? ntok - c - (lane >> 4) : 0;  // tokens of this lane's parity from here on
+          if (p.act == RF_ACT_SILU) store_gated<T, RF_ACT_SILU>(v, lane, out, p.N, left);
+          else if (p.act == RF_ACT_GELU) store_gated<T, RF_ACT_GELU>(v, lane, out, p.N, left);
+          else store_gated<T, RF_ACT_GELU_TANH>(v, lane, out, p.N, left);
         } else {
           float *out = reinterpret_cast<float *>(p.out) + (int64_t)(row0 + c) * p.N + f;
+          const int left = f < p.N ? ntok - c : 0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < ntok && f < p.N) out[(int64_t)i * p.N] = __uint_as_float(v[i]);
+          for (int i = 0; i < 16; ++i, out += p.N)
+            if (i < left) *out = __uint_as_float(v[i]);
         }
       }
     }

@@ -124,13 +124,19 @@ template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_
 template <typename T, int ACT>
 __device__ __forceinline__ void store_gated(const uint32_t (&v)[16], int lane, T *out, int N, int left) {
   const bool up = lane >= 16;
+  float h[8];  // eight chains at a time: inside the stores' conditions they ran one after another
 #pragma unroll
-  for (int i = 0; i < 8; ++i, out += 2 * (int64_t)N) {
+  for (int i = 0; i < 8; ++i) {
     const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? v[2 * i] : v[2 * i + 1], 16);
     const float g = __uint_as_float(up ? got : v[2 * i]);
     const float u = __uint_as_float(up ? v[2 * i + 1] : got);
-    if (2 * i < left) *out = rf::Cvt<T>::from_f(rf::act_gate_t<ACT>(g) * u);
+    h[i] = rf::act_gate_t<ACT>(g) * u;
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(h[i]));
+#pragma unroll
+  for (int i = 0; i < 8; ++i, out += 2 * (int64_t)N)
+    if (2 * i < left) *out = rf::Cvt<T>::from_f(h[i]);
 }
 
 // SUBS: scale groups in a stage's 128 k (1, 2 or 4).
@@ -351,6 +357,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         uint32_t v[16];
         tmem_ld16(tb + (uint32_t)c, v);
         tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));  // no use of v moves above the wait
         if (c + 16 >= np) {  // the accumulator is free for the pair's tile after next
           tc_fence_before();
           __syncwarp();

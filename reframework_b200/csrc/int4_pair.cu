@@ -107,6 +107,33 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
+// sw128_desc of an address, its low word; the high word is the same for all.
+constexpr uint32_t SW128_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ void tc_mma_pair_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SW128_DESC_HI)
+      : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once all MMAs issued so far have completed.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 // Two 16-bit products, each rounded to nearest (exact for short scales).
 template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
@@ -291,10 +318,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---------------------------------------------------------- MMA issuer
+      // The whole warp walks the loop and one elected lane issues: addresses
+      // and descriptors stay warp-uniform (inside a one-lane branch an MMA took
+      // 88 cycles to issue, most of it moving its operands to uniform registers).
       const uint32_t IDESC = pair_idesc_base<T>();
-      const uint32_t peer_bars = mapa_shared(bar0, 1);
+      const uint32_t a_desc = sw128_desc_lo(smem_u32(sA)), b_desc = sw128_desc_lo(smem_u32(sB));
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -303,37 +333,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         decode(t, e, row0, ntok, fb);
         const uint32_t idesc = IDESC | ((uint32_t)(((ntok + 15) & ~15) >> 3) << 17);
         const int acc = it & 1;
-        if (!pwait(TEMPTY(acc), (uint32_t)(((it >> 1) & 1) ^ 1), 0)) break;
+        ok = __all_sync(0xffffffffu, pwait(TEMPTY(acc), (uint32_t)(((it >> 1) & 1) ^ 1), 0));
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(acc * 256);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!pwait(FULL(stage), phase, 0)) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, pwait(FULL(stage), phase, 0));
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * Q_KSUB * Q_A_SUB);
-          const uint32_t b0 = smem_u32(sB + stage * Q_KSUB * Q_B_SUB);
+          const uint32_t a0 = a_desc + (uint32_t)(stage * (Q_KSUB * Q_A_SUB >> 4));
+          const uint32_t b0 = b_desc + (uint32_t)(stage * (Q_KSUB * Q_B_SUB >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < Q_KSUB; ++j)
+            for (int j = 0; j < Q_KSUB; ++j)
 #pragma unroll
-            for (int k = 0; k < Q_BK / 16; ++k)
-              tc_mma_pair(d, sw128_desc(a0 + j * Q_A_SUB + k * 32), sw128_desc(b0 + j * Q_B_SUB + k * 32), idesc,
-                          (kb | j | k) ? 1u : 0u);
-          tc_commit_pair(EMPTY(stage));  // frees the stage in both CTAs once read
-          tc_commit_pair(peer_bars + (EMPTY(stage) - bar0));
+              for (int k = 0; k < Q_BK / 16; ++k)
+                tc_mma_pair_lo(d, a0 + (uint32_t)((j * Q_A_SUB + k * 32) >> 4), b0 + (uint32_t)((j * Q_B_SUB + k * 32) >> 4),
+                               idesc, (kb | j | k) ? 1u : 0u);
+            tc_commit_both(EMPTY(stage));  // frees the stage in both CTAs once read
+            if (kb == num_kb - 1) tc_commit_both(TFULL(acc));
+          }
+          __syncwarp();
           if (++stage == Q_STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (!ok) break;
-        tc_commit_pair(TFULL(acc));
-        tc_commit_pair(peer_bars + (TFULL(acc) - bar0));
       }
       // no MMA may still be running when either CTA releases TMEM or exits
-      tc_commit_pair(DRAIN);
-      mbar_wait_teardown(DRAIN, 0);
+      if (elect_one()) {
+        tc_commit_pair(DRAIN);
+        mbar_wait_teardown(DRAIN, 0);
+      }
+      __syncwarp();
     }
   } else if (warp < 2 + Q_EPI_WARPS) {
     // ------------------------------------------------------------ epilogue

@@ -282,40 +282,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------- token producer
-    if (lane == 0) {
-      const uint32_t full0 = mapa_shared(FULL(0), 0);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = pair; t < total && ok; t += npairs) {
-        int e, row0, ntok, fb;
-        decode(t, e, row0, ntok, fb);
-        const int half = ((ntok + 15) & ~15) >> 1;  // token rows per CTA: a multiple of 8
-        int bi = 0;
-        while ((8 << bi) < half) ++bi;
-        const uint32_t bytes = (uint32_t)Q_KSUB * (uint32_t)(8 << bi) * (Q_BK * 2);  // per CTA
-        const int xrow = row0 + (rank ? half : 0);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!pwait(EMPTY(stage), phase ^ 1u, 0)) {
-            ok = false;
-            break;
-          }
+    const uint32_t full0 = mapa_shared(FULL(0), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = pair; t < total && ok; t += npairs) {
+      int e, row0, ntok, fb;
+      decode(t, e, row0, ntok, fb);
+      const int half = ((ntok + 15) & ~15) >> 1;  // token rows per CTA: a multiple of 8
+      int bi = 0;
+      while ((8 << bi) < half) ++bi;
+      const uint32_t bytes = (uint32_t)Q_KSUB * (uint32_t)(8 << bi) * (Q_BK * 2);  // per CTA
+      const int xrow = row0 + (rank ? half : 0);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = __all_sync(0xffffffffu, pwait(EMPTY(stage), phase ^ 1u, 0));
+        if (!ok) break;
+        if (elect_one()) {
           const uint32_t b_dst = smem_u32(sB + stage * Q_KSUB * Q_B_SUB);
           if (rank == 0) mbar_expect_tx(FULL(stage), 2u * bytes);  // both CTAs load the same box sizes
 #pragma unroll
           for (int j = 0; j < Q_KSUB; ++j)
             tma_load_2d_pair(b_dst + (uint32_t)(j * Q_B_SUB), &tmX.m[bi], full0 + 8u * (uint32_t)stage,
                              (kb * Q_KSUB + j) * Q_BK, xrow);
-          if (++stage == Q_STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (++stage == Q_STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
-        const uint64_t t0 = rf::globaltimer_ns();
-        while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
-      }
+    }
+    if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
+      const uint64_t t0 = rf::globaltimer_ns();
+      while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -413,23 +412,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     }
   } else if (warp == Q_COPY_WARP) {
     // ---------------------------------------------- codes and scales producer
-    if (lane == 0) {
-      const int64_t row_blocks = p.sh.row_blocks();
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = pair; t < total && ok; t += npairs) {
-        int e, row0, ntok, fb;
-        decode(t, e, row0, ntok, fb);
-        // two boxes of four row blocks: gate and up, or eight in a row; blocks
-        // past the weight's own are some other rows or zeros, never stored
-        const int rb0 = (int)((int64_t)e * row_blocks) + (GATED ? fb * 8 + (int)rank * 4 : fb * 16 + (int)rank * 8);
-        const int rb1 = rb0 + (GATED ? (int)p.sh.half_blocks : 4);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!pwait(CEMPTY(stage), phase ^ 1u, 0)) {
-            ok = false;
-            break;
-          }
+    const int64_t row_blocks = p.sh.row_blocks();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = pair; t < total && ok; t += npairs) {
+      int e, row0, ntok, fb;
+      decode(t, e, row0, ntok, fb);
+      // two boxes of four row blocks: gate and up, or eight in a row; blocks past
+      // the weight's own are some other rows or zeros, never stored
+      const int rb0 = (int)((int64_t)e * row_blocks) + (GATED ? fb * 8 + (int)rank * 4 : fb * 16 + (int)rank * 8);
+      const int rb1 = rb0 + (GATED ? (int)p.sh.half_blocks : 4);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = __all_sync(0xffffffffu, pwait(CEMPTY(stage), phase ^ 1u, 0));
+        if (!ok) break;
+        if (elect_one()) {
           const uint32_t dst = smem_u32(sQ) + (uint32_t)(stage * (Q_CODE_BYTES + Q_SCALE_BYTES));
           const uint32_t sdst = dst + Q_CODE_BYTES;
           mbar_expect_tx(CFULL(stage), Q_CODE_BYTES + Q_BLOCKS * SUBS * rf::I4_ROWS * 2);
@@ -437,16 +434,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
           tma_load_2d(dst + Q_CODE_BYTES / 2, &tmW, CFULL(stage), kb * (Q_KSUB * rf::I4_BLOCK / 4), rb1);
           tma_load_2d(sdst, &tmS, CFULL(stage), kb * (SUBS * rf::I4_ROWS), rb0);
           tma_load_2d(sdst + Q_SCALE_BYTES / 2, &tmS, CFULL(stage), kb * (SUBS * rf::I4_ROWS), rb1);
-          if (++stage == Q_STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (++stage == Q_STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
-        const uint64_t t0 = rf::globaltimer_ns();
-        while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
-      }
+    }
+    if (!ok) {  // let the copies in flight land before this CTA can exit (bounded pause)
+      const uint64_t t0 = rf::globaltimer_ns();
+      while (rf::globaltimer_ns() - t0 < Q_ABORT_DRAIN_NS) __nanosleep(1000);
     }
   } else {
     // --------------------------------------------------------- code warps

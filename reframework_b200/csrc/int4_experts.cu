@@ -6,16 +6,23 @@
 // for the rows r that the permute gives expert e.  h is rounded because it is
 // the second product's 16-bit operand; everything else stays fp32 up to out.
 //
-// Few rows per expert (int4_skinny_kernel): bound by reading the weights, half
-// a byte each.  A block takes 32 weight rows (gated: 16 gate and their 16 up
-// rows) of one expert over the whole reduction, its eight warps one eighth of
-// it each; a lane's 16-byte word of the stored layout is its fragment of four
-// 16 x 16 tiles of mma.sync, the codes as exact 16-bit integers, and the
-// tokens (8 to a tile) are read straight from their rows.  A group's sums are
-// scaled in fp32 after its products.  The eight partial sums meet in shared
-// memory in warp order, so results do not depend on timing.
+// Few pairs (T * K <= 1024, few rows per expert): int4_few_kernel, bound by
+// reading the weights, half a byte each, and close behind by the instructions
+// that unpack them.  A block takes 32 weight rows at a time (gated: 16 gate and
+// their 16 up rows) of one expert over the whole reduction, its eight warps an
+// eighth of it each; a lane's 16-byte word of the stored layout is its fragment
+// of four 16 x 16 tiles of mma.sync, the codes as exact 16-bit integers, and
+// the tokens (8 or 16 at a time) are read straight from their rows.  A group's
+// sums are scaled in fp32 after its products.  The eight partial sums meet in
+// shared memory in warp order, so results do not depend on timing.  There is no
+// permutation: every block finds its expert's pairs in the ids, h and y rows
+// are the pairs themselves, and the three launches (gated, down, combine) are
+// chained by programmatic dependent launch, each waiting for its predecessor's
+// rows only after its ids and first weights are on the way.
+// Many rows per expert: permute with the row gather, then int4_pair.cu.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "gemm.cuh"
 #include "int4.cuh"
@@ -24,37 +31,36 @@ RF_DEVICE_ERROR_WORD();
 
 namespace {
 
-constexpr int SK_WARPS = 8;
-constexpr int SK_THREADS = SK_WARPS * 32;
-constexpr int SK_UNROLL = 4;  // k blocks whose loads are in flight together
+constexpr int FW_WARPS = 8;
+constexpr int FW_THREADS = FW_WARPS * 32;
+constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
+constexpr int FW_STEP = 128;    // k per step: two blocks of codes
 constexpr int KMAX = 16;
 
-struct SkinnyArgs {
-  const void *a;        // x [tokens, Kd] (gated) or h [rows, Kd]
+struct FewArgs {
+  const void *a;         // x [T, Kd] (gated) or h [pairs, Kd]
   const uint8_t *w;
   const void *scales;
-  void *out;            // h [rows, N] in T (gated) or y [rows, N] fp32
-  const int32_t *offsets, *counts;
-  const int32_t *src;   // gated: row -> token * topk + slot
-  int topk, E, N, Kd, group, act;
+  void *out;             // h [pairs, N] in T (gated) or y [pairs, N] fp32
+  const int32_t *ids;    // [pairs]
+  int pairs, topk, E, N, Kd, act, units;
   rf::Int4Shape sh;
 };
 
+// d = a . b + (first ? 0 : d)
 template <typename T>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 __device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {  // weights pass through once: not kept in L1
@@ -64,184 +70,282 @@ __device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {  // weights pass t
                : "l"(p));
   return v;
 }
-
-// The y-th expert (ascending) that has rows, or -1.
-__device__ __forceinline__ int nth_active(const int32_t *counts, int E, int y) {
-  const int lane = threadIdx.x & 31;
-  for (int c = 0; c < E; c += 32) {
-    const unsigned b = __ballot_sync(0xffffffffu, c + lane < E && counts[c + lane] > 0);
-    const int n = __popc(b);
-    if (y < n) return c + (int)__fns(b, 0, y + 1);
-    y -= n;
-  }
-  return -1;
-}
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Waits until the launch before this one is complete and its writes visible.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Two neighbouring 16-bit scales (rows r and r + 8) as floats.
 template <typename T>
 __device__ __forceinline__ float2 scale_pair(uint32_t v) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-  } else {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
-// SUB: scale groups in a 64-k block (2 for groups of 32, else 1).
-template <typename T, int NT, bool GATED, int SUB>
-__global__ void __launch_bounds__(SK_THREADS) int4_skinny_kernel(const SkinnyArgs p) {
-  __shared__ float red[SK_WARPS][2 * NT * 4 * 32];
+struct FewShared {
+  float red[FW_WARPS][2 * 2 * 4 * 32];
+  int list[FW_PAIRS];       // this expert's pairs, ascending
+  uint32_t active[32];      // one bit per expert with a pair
+  int expert, count, part[FW_WARPS];
+};
+
+// The y-th expert (ascending) that some pair names, its pairs into s.list and
+// their number; expert -1 if there are not so many.
+__device__ __forceinline__ void find_expert(const FewArgs &p, FewShared &s, int y, bool report) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 32) s.active[tid] = 0u;
+  if (tid == 0) s.count = 0;
+  int id[FW_PAIRS / FW_THREADS];
+#pragma unroll
+  for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i) {
+    const int at = i * FW_THREADS + tid;
+    id[i] = at < p.pairs ? p.ids[at] : -1;
+    if (at < p.pairs && (unsigned)id[i] >= (unsigned)p.E) {
+      if (report) rf_report(RF_DEV_BAD_EXPERT_ID);
+      id[i] = -1;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i)
+    if (id[i] >= 0) atomicOr(&s.active[id[i] >> 5], 1u << (id[i] & 31));
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t bits = s.active[lane];
+    const int n = __popc(bits);
+    int before = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
+    }
+    before -= n;
+    if (lane == 31 && y >= before + n) s.expert = -1;
+    if (y >= before && y < before + n) s.expert = lane * 32 + (int)__fns(bits, 0, y - before + 1);
+  }
+  __syncthreads();
+  const int e = s.expert;
+  if (e < 0) return;
+#pragma unroll
+  for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i) {
+    if (i * FW_THREADS >= p.pairs) break;
+    const unsigned b = __ballot_sync(0xffffffffu, id[i] == e);
+    if (lane == 0) s.part[warp] = __popc(b);
+    __syncthreads();
+    int base = s.count, all = 0;
+#pragma unroll
+    for (int w = 0; w < FW_WARPS; ++w) {
+      base += w < warp ? s.part[w] : 0;
+      all += s.part[w];
+    }
+    if (id[i] == e) s.list[base + __popc(b & ((1u << lane) - 1u))] = i * FW_THREADS + tid;
+    __syncthreads();
+    if (tid == 0) s.count += all;
+  }
+  __syncthreads();
+}
+
+// One step's operands in registers.
+template <int NT, int SUBS>
+struct FewStep {
+  uint4 q[2][2];         // [row block][block of 64 k]
+  uint32_t s[2][SUBS];
+  uint4 x[NT][2][2];     // [8 tokens][block][half]
+};
+
+// 32 weight rows x 8 NT tokens of the expert (from pair c0 of the list on).
+// SUBS: scale groups in a step's 128 k (1, 2 or 4).
+template <typename T, bool GATED, int SUBS, int NT>
+__device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e, int unit, int c0, bool &waited) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int e = nth_active(p.counts, p.E, blockIdx.y);
-  if (e < 0) return;
-  const int row0 = p.offsets[e], cnt = p.counts[e];
-  const int unit = blockIdx.x;
+  const int cnt = sm.count;
   const int KB = (int)p.sh.k_blocks, groups = (int)p.sh.groups;
-  const int64_t rb1 = GATED ? p.sh.half_blocks + unit : min((int64_t)(2 * unit + 1), p.sh.row_blocks() - 1);
+  const int steps = (KB + 1) / 2;
+  const int st0 = steps * warp / FW_WARPS, st1 = steps * (warp + 1) / FW_WARPS;
   const uint4 *wp[2];
   const uint32_t *sp[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int64_t b = (int64_t)e * p.sh.row_blocks() + (r ? rb1 : (int64_t)(GATED ? unit : 2 * unit));
-    wp[r] = reinterpret_cast<const uint4 *>(p.w + b * KB * rf::I4_BLOCK) + lane;
-    sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) + b * groups * rf::I4_ROWS) + g;
+    int64_t rb = GATED ? unit + r * p.sh.half_blocks : 2 * (int64_t)unit + r;
+    rb = (int64_t)e * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
+    wp[r] = reinterpret_cast<const uint4 *>(p.w + rb * KB * rf::I4_BLOCK) + lane;
+    sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) + rb * groups * rf::I4_ROWS) + g;
   }
-  const int kb0 = KB * warp / SK_WARPS, kb1 = KB * (warp + 1) / SK_WARPS;
-  const T *a = reinterpret_cast<const T *>(p.a);
-  for (int c0 = 0; c0 < cnt; c0 += 8 * NT) {
-    const T *xp[NT];
+  const T *xp[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = c0 + 8 * n + g;
-      xp[n] = nullptr;
-      if (r < cnt) xp[n] = a + (int64_t)(GATED ? p.src[row0 + r] / p.topk : row0 + r) * p.Kd;
+  for (int n = 0; n < NT; ++n) {
+    const int i = c0 + 8 * n + g;
+    const int pair = i < cnt ? sm.list[i] : -1;
+    xp[n] = pair < 0 ? nullptr : reinterpret_cast<const T *>(p.a) + (int64_t)(GATED ? pair / p.topk : pair) * p.Kd + 8 * c;
+  }
+  auto load_weights = [&](FewStep<NT, SUBS> &f, int st) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)  // codes past the last block meet zero token values
+        f.q[r][b] = ldg_stream(wp[r] + (int64_t)min(2 * st + b, KB - 1) * 32);
+#pragma unroll
+      for (int i = 0; i < SUBS; ++i) f.s[r][i] = __ldg(sp[r] + (int64_t)min(st * SUBS + i, groups - 1) * 8);
     }
-    float acc[2][NT][4];
+  };
+  auto load_tokens = [&](FewStep<NT, SUBS> &f, int st) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.f;
-    for (int kb = kb0; kb < kb1; kb += SK_UNROLL) {
-      uint4 q[SK_UNROLL][2], x[SK_UNROLL][NT][2];
-      uint32_t s[SK_UNROLL][2][SUB];
+        for (int h = 0; h < 2; ++h) {
+          const int k = st * FW_STEP + 64 * b + 32 * h;
+          f.x[n][b][h] = xp[n] && k + 8 * c < p.Kd ? *reinterpret_cast<const uint4 *>(xp[n] + k) : make_uint4(0u, 0u, 0u, 0u);
+        }
+  };
+  float acc[2][NT][4];
 #pragma unroll
-      for (int u = 0; u < SK_UNROLL; ++u) {
-        const bool in = kb + u < kb1;
-        const int k = (kb + u) * rf::I4_K;
+  for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          q[u][r] = in ? ldg_stream(wp[r] + (int64_t)(kb + u) * 32) : make_uint4(0u, 0u, 0u, 0u);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int h = 0; h < SUB; ++h) {
-            const int gr = (k + 32 * h) / p.group;  // past the last group only where the codes are padding
-            s[u][r][h] = in && gr < groups ? __ldg(sp[r] + (int64_t)gr * 8) : 0u;
+      for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.f;
+  auto multiply = [&](const FewStep<NT, SUBS> &f) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float d[NT][4];
+#pragma unroll
+      for (int hh = 0; hh < 4; ++hh) {  // 32 k each
+        const int b = hh >> 1, h = hh & 1;
+        const uint32_t lo = h ? f.q[r][b].y : f.q[r][b].x, hi = h ? f.q[r][b].w : f.q[r][b].z;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint32_t fr[4] = {rf::int4_pair<T>(lo, 2 * m), rf::int4_pair<T>(hi, 2 * m),
+                                  rf::int4_pair<T>(lo, 2 * m + 1), rf::int4_pair<T>(hi, 2 * m + 1)};
+          const bool first = m == 0 && hh % (4 / SUBS) == 0;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 xv = f.x[n][b][h];
+            mma_16816<T>(d[n], fr, m ? xv.z : xv.x, m ? xv.w : xv.y, first);
           }
         }
+        if ((hh + 1) % (4 / SUBS) == 0) {
+          const float2 sc = scale_pair<T>(f.s[r][hh / (4 / SUBS)]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int kx = k + 32 * h + 8 * c;
-            x[u][n][h] = in && xp[n] && kx < p.Kd ? __ldg(reinterpret_cast<const uint4 *>(xp[n] + kx))
-                                                 : make_uint4(0u, 0u, 0u, 0u);
-          }
-      }
-#pragma unroll
-      for (int u = 0; u < SK_UNROLL; ++u) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float d[NT][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // the block's halves: words h of rows g and g + 8
-            if (h == 0 || SUB == 2) {
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) d[n][j] = 0.f;
-            }
-            const uint32_t lo = h ? q[u][r].y : q[u][r].x, hi = h ? q[u][r].w : q[u][r].z;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              const uint32_t fr[4] = {rf::int4_pair<T>(lo, 2 * m), rf::int4_pair<T>(hi, 2 * m),
-                                      rf::int4_pair<T>(lo, 2 * m + 1), rf::int4_pair<T>(hi, 2 * m + 1)};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint4 xv = x[u][n][h];
-                mma_16816<T>(d[n], fr, m ? xv.z : xv.x, m ? xv.w : xv.y);
-              }
-            }
-            if (h == 1 || SUB == 2) {
-              const float2 f = scale_pair<T>(s[u][r][SUB == 2 ? h : 0]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                acc[r][n][0] = fmaf(d[n][0], f.x, acc[r][n][0]);
-                acc[r][n][1] = fmaf(d[n][1], f.x, acc[r][n][1]);
-                acc[r][n][2] = fmaf(d[n][2], f.y, acc[r][n][2]);
-                acc[r][n][3] = fmaf(d[n][3], f.y, acc[r][n][3]);
-              }
-            }
+          for (int n = 0; n < NT; ++n) {
+            acc[r][n][0] = fmaf(d[n][0], sc.x, acc[r][n][0]);
+            acc[r][n][1] = fmaf(d[n][1], sc.x, acc[r][n][1]);
+            acc[r][n][2] = fmaf(d[n][2], sc.y, acc[r][n][2]);
+            acc[r][n][3] = fmaf(d[n][3], sc.y, acc[r][n][3]);
           }
         }
       }
     }
-    // ---- the warps' partial sums, in warp order
-    __syncthreads();  // the previous chunk's sums have been read
+  };
+  FewStep<NT, SUBS> fa, fb;  // the next step is on its way while one is multiplied
+  if (st0 < st1) load_weights(fa, st0);
+  if (!waited) {
+    wait_for_previous();  // the rows of h come from the launch before
+    waited = true;
+  }
+  if (st0 < st1) load_tokens(fa, st0);
+  for (int st = st0; st < st1; st += 2) {
+    if (st + 1 < st1) {
+      load_weights(fb, st + 1);
+      load_tokens(fb, st + 1);
+    }
+    multiply(fa);
+    if (st + 1 >= st1) break;
+    if (st + 2 < st1) {
+      load_weights(fa, st + 2);
+      load_tokens(fa, st + 2);
+    }
+    multiply(fb);
+  }
+  // ---- the warps' partial sums, in warp order
+  __syncthreads();  // the previous pass's sums have been read
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+  for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) red[warp][((r * NT + n) * 4 + j) * 32 + lane] = acc[r][n][j];
-    __syncthreads();
-    constexpr int PER = GATED ? 16 : 32;  // features of a unit
-    for (int i = threadIdx.x; i < PER * 8 * NT; i += SK_THREADS) {
-      const int f = i % PER, col = i / PER;  // feature, token of the chunk
-      const int r16 = f & 15;
-      const int at = ((col >> 3) * 4 + (col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + ((col & 7) >> 1);
-      if (c0 + col >= cnt) continue;
-      const int64_t row = row0 + c0 + col;
-      if constexpr (GATED) {
-        float gt = 0.f, up = 0.f;
+      for (int j = 0; j < 4; ++j) sm.red[warp][((r * NT + n) * 4 + j) * 32 + lane] = acc[r][n][j];
+  __syncthreads();
+  constexpr int PER = GATED ? 16 : 32;  // features of a unit
+  for (int i = threadIdx.x; i < PER * 8 * NT; i += FW_THREADS) {
+    const int f = i % PER, col = i / PER;  // feature, token of the pass
+    const int r16 = f & 15;
+    const int at = ((col >> 3) * 4 + (col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + ((col & 7) >> 1);
+    const int64_t feat = (int64_t)unit * PER + f;
+    if (c0 + col >= cnt || feat >= p.N) continue;
+    const int64_t row = sm.list[c0 + col];
+    if constexpr (GATED) {
+      float gt = 0.f, up = 0.f;
 #pragma unroll
-        for (int w = 0; w < SK_WARPS; ++w) {
-          gt += red[w][at];
-          up += red[w][at + NT * 4 * 32];
-        }
-        const int64_t feat = (int64_t)unit * 16 + f;
-        if (feat < p.N) reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
-      } else {
-        float y = 0.f;
-#pragma unroll
-        for (int w = 0; w < SK_WARPS; ++w) y += red[w][at + (f >> 4) * NT * 4 * 32];
-        const int64_t feat = (int64_t)unit * 32 + f;
-        if (feat < p.N) reinterpret_cast<float *>(p.out)[row * p.N + feat] = y;
+      for (int w = 0; w < FW_WARPS; ++w) {
+        gt += sm.red[w][at];
+        up += sm.red[w][at + NT * 4 * 32];
       }
+      reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
+    } else {
+      float y = 0.f;
+#pragma unroll
+      for (int w = 0; w < FW_WARPS; ++w) y += sm.red[w][at + (f >> 4) * NT * 4 * 32];
+      reinterpret_cast<float *>(p.out)[row * p.N + feat] = y;
     }
   }
 }
 
-template <typename T, int NT>
-int launch_skinny_t(const SkinnyArgs &p, bool gated, int max_active, cudaStream_t st) {
-  const int units = (int)(gated ? p.sh.half_blocks : (p.sh.row_blocks() + 1) / 2);
-  const dim3 grid(units, max_active);
-  if (gated) {
-    if (p.group == 32) int4_skinny_kernel<T, NT, true, 2><<<grid, SK_THREADS, 0, st>>>(p);
-    else int4_skinny_kernel<T, NT, true, 1><<<grid, SK_THREADS, 0, st>>>(p);
-  } else {
-    if (p.group == 32) int4_skinny_kernel<T, NT, false, 2><<<grid, SK_THREADS, 0, st>>>(p);
-    else int4_skinny_kernel<T, NT, false, 1><<<grid, SK_THREADS, 0, st>>>(p);
+template <typename T, bool GATED, int SUBS>
+__global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
+  __shared__ FewShared sm;
+  launch_dependents();
+  find_expert(p, sm, blockIdx.y, GATED && blockIdx.x == 0 && blockIdx.y == 0);
+  const int e = sm.expert;
+  if (e < 0) return;
+  bool waited = GATED;
+  const int cnt = sm.count;
+  for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    for (int c0 = 0; c0 < cnt; c0 += 8) few_pass<T, GATED, SUBS, 1>(p, sm, e, unit, c0, waited);
   }
-  return rf::check_launch(gated ? "4-bit gated products" : "4-bit down products");
 }
 
-int launch_skinny(const rf::Int4Gemm &g, bool gated, const int32_t *src, int topk, int max_active, cudaStream_t st) {
-  const SkinnyArgs p{g.a, g.w, g.scales, g.out, g.offsets, g.counts, src, topk, g.E, g.N, g.Kdim, g.group, g.act,
-                     rf::int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated)};
-  if (g.dtype == RF_F16) return launch_skinny_t<__half, 1>(p, gated, max_active, st);
-  return launch_skinny_t<__nv_bfloat16, 1>(p, gated, max_active, st);
+// Launches `kern` so that it may start while the previous launch on the stream
+// drains (it waits for it itself, wait_for_previous).
+template <typename... Params, typename... Args>
+int launch_chained(const char *what, void (*kern)(Params...), dim3 grid, int threads, bool chained, cudaStream_t st,
+                   Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, Params(args)...);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return rf::fail(RF_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
+  }
+  return RF_OK;
+}
+
+template <typename T, bool GATED>
+int launch_few_t(const FewArgs &p, int group, dim3 grid, cudaStream_t st) {
+  const char *what = GATED ? "4-bit gated products (few rows)" : "4-bit down products (few rows)";
+  if (group == 32) return launch_chained(what, int4_few_kernel<T, GATED, 4>, grid, FW_THREADS, !GATED, st, p);
+  if (group == 64) return launch_chained(what, int4_few_kernel<T, GATED, 2>, grid, FW_THREADS, !GATED, st, p);
+  return launch_chained(what, int4_few_kernel<T, GATED, 1>, grid, FW_THREADS, !GATED, st, p);
+}
+
+int launch_few(const rf::Int4Gemm &g, bool gated, const int32_t *ids, int topk, cudaStream_t st) {
+  const rf::Int4Shape sh = rf::int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated);
+  const int units = (int)(gated ? sh.half_blocks : (sh.row_blocks() + 1) / 2);
+  const FewArgs p{g.a, g.w, g.scales, g.out, ids, (int)g.rows, topk, g.E, g.N, g.Kdim, g.act, units, sh};
+  // a block per unit and expert, fewer where that is more than eight waves
+  const int active = (int)std::min<int64_t>(g.E, g.rows);
+  const int most = std::max(1, rf::num_sms() * 16 / active);
+  const dim3 grid((unsigned)std::min(units, most), (unsigned)active);
+  if (g.dtype == RF_F16) return gated ? launch_few_t<__half, true>(p, g.group, grid, st) : launch_few_t<__half, false>(p, g.group, grid, st);
+  return gated ? launch_few_t<__nv_bfloat16, true>(p, g.group, grid, st) : launch_few_t<__nv_bfloat16, false>(p, g.group, grid, st);
 }
 
 // ------------------------------------------------------------------ combine
@@ -249,14 +353,15 @@ constexpr int CB_THREADS = 128;
 
 struct CombineArgs {
   const float *y;
-  const int32_t *row_of_slot;
+  const int32_t *row_of_slot;  // y's row of a pair (-1: none), or
+  const int32_t *ids;          // the pair itself unless its id names no expert
   const float *w;
   const void *shared_y;
   const float *shared_scale;
   const void *residual;
   void *out;
   int64_t T;
-  int K, H;
+  int K, H, E;
 };
 
 // One block per (token, 128 * 8 columns): fp32 sums in slot order, one
@@ -264,17 +369,20 @@ struct CombineArgs {
 template <typename T>
 __global__ void __launch_bounds__(CB_THREADS) int4_combine_kernel(const CombineArgs a) {
   const int col = (blockIdx.y * CB_THREADS + threadIdx.x) * 8;
+  wait_for_previous();
   if (col >= a.H) return;
   for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
     float acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     for (int k = 0; k < a.K; ++k) {
-      const int r = a.row_of_slot[t * a.K + k];
+      int64_t r = t * a.K + k;
+      if (a.ids) r = (unsigned)a.ids[r] < (unsigned)a.E ? r : -1;
+      else r = a.row_of_slot[r];
       if (r < 0) continue;  // an id that names no expert
       const float w = a.w[t * a.K + k];
-      const float4 *p = reinterpret_cast<const float4 *>(a.y + (int64_t)r * a.H + col);
-      const float4 u = __ldg(p), v = __ldg(p + 1);
+      const float4 *p = reinterpret_cast<const float4 *>(a.y + r * a.H + col);
+      const float4 u = p[0], v = p[1];
       const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
@@ -302,8 +410,8 @@ template <typename T>
 int launch_combine(const CombineArgs &a, cudaStream_t st) {
   const int64_t gy = (a.H + CB_THREADS * 8 - 1) / (CB_THREADS * 8);
   const int64_t gx = std::min<int64_t>(a.T, std::max<int64_t>(1, (int64_t)rf::num_sms() * 16 / gy));
-  int4_combine_kernel<T><<<dim3((unsigned)gx, (unsigned)gy), CB_THREADS, 0, st>>>(a);
-  return rf::check_launch("4-bit combine");
+  return launch_chained("4-bit combine", int4_combine_kernel<T>, dim3((unsigned)gx, (unsigned)gy), CB_THREADS, a.ids != nullptr,
+                        st, a);
 }
 
 // ------------------------------------------------------------------ workspace
@@ -347,8 +455,8 @@ constexpr int64_t PAIR_ROWS = 8;
 
 bool use_pair(int64_t T, int64_t K, int64_t E) {
   const int impl = rf::gemm_impl();
+  if (T * K > FW_PAIRS || impl == 5) return true;
   if (impl == 1) return false;
-  if (impl == 5) return true;
   return T * K >= PAIR_ROWS * std::min(E, T * K);
 }
 
@@ -386,18 +494,22 @@ extern "C" int rf_moe_int4_experts(const void *x, int dtype, const void *w1, con
   int32_t *ros = (int32_t *)(ws + l.row_of_slot), *src = (int32_t *)(ws + l.src);
   cudaStream_t st = (cudaStream_t)stream;
   const bool pair = use_pair(T, K, E);
-  int rc = rf_moe_permute(topk_ids, T, K, E, 1, pair ? x : nullptr, dtype, pair ? H : 0, offsets, counts, ros, src,
-                          pair ? ws + l.x : nullptr, ws + l.permute, l.permute_bytes, stream);
-  if (rc) return rc;
   const rf::Int4Gemm g{pair ? ws + l.x : x, (const uint8_t *)w1, w1_scales, ws + l.h, offsets, counts, l.rows, (int)E,
                        (int)H, (int)I, (int)w1_group, dtype, activation};
   const rf::Int4Gemm d{ws + l.h, (const uint8_t *)w2, w2_scales, ws + l.y, offsets, counts, l.rows, (int)E,
                        (int)I, (int)H, (int)w2_group, dtype, activation};
-  const int max_active = (int)std::min<int64_t>(E, T * K);
-  rc = pair ? rf::launch_int4_pair(g, true, st) : launch_skinny(g, true, src, (int)K, max_active, st);
+  int rc;
+  if (pair) {
+    rc = rf_moe_permute(topk_ids, T, K, E, 1, x, dtype, H, offsets, counts, ros, src, ws + l.x, ws + l.permute,
+                        l.permute_bytes, stream);
+    if (!rc) rc = rf::launch_int4_pair(g, true, st);
+    if (!rc) rc = rf::launch_int4_pair(d, false, st);
+  } else {
+    rc = launch_few(g, true, topk_ids, (int)K, st);
+    if (!rc) rc = launch_few(d, false, topk_ids, 1, st);
+  }
   if (rc) return rc;
-  rc = pair ? rf::launch_int4_pair(d, false, st) : launch_skinny(d, false, nullptr, 1, max_active, st);
-  if (rc) return rc;
-  const CombineArgs cb{(const float *)(ws + l.y), ros, topk_weights, shared_y, shared_scale, residual, out, T, (int)K, (int)H};
+  const CombineArgs cb{(const float *)(ws + l.y), pair ? ros : nullptr, pair ? nullptr : topk_ids, topk_weights, shared_y,
+                       shared_scale, residual, out, T, (int)K, (int)H, (int)E};
   return dtype == RF_F16 ? launch_combine<__half>(cb, st) : launch_combine<__nv_bfloat16>(cb, st);
 }

@@ -3,8 +3,9 @@
 //
 // A weight is scale[n, k / g] * (code[n, k] - 8), code in 0..15, g in
 // {32, 64, 128} along the reduction axis.  Stored per expert slot:
-//   data   [row blocks][k blocks][512 bytes]   16 rows x 64 k to a block
-//   scales [row blocks][groups][16]            in the layer dtype
+//   data   [row blocks][k blocks][512 bytes]        16 rows x 64 k to a block
+//   scales [row blocks][steps][8][128 / g][2]       in the layer dtype
+// with an even number of k blocks, two to a step of 128 k,
 // so that a warp reads a block as 32 consecutive 16-byte words.  Lane
 // 4 * r + c (r = 0..7, c = 0..3) holds, as four 32-bit words of 8 codes: row
 // r's k = 8 c .. 8 c + 7, its k = 32 + 8 c .. 32 + 8 c + 7, and the same of row
@@ -13,8 +14,8 @@
 // half of the block (a scale group of 32 is a half), and four 16-byte pieces
 // of a K-major shared-memory tile.  In a word, code 2 i sits in nibble i and
 // code 2 i + 1 in nibble i + 4, so that one shift and one mask give the
-// neighbouring pair as two 16-bit halves.  The scales of rows r and r + 8 are
-// neighbours (entry 2 r + h).
+// neighbouring pair as two 16-bit halves.  The scales of a step are stored row r
+// = 0..7 first, then group, then row r or r + 8: a lane's are one word to 16 bytes.
 // Rows and k past the weight's own are stored as code 8 (zero) with scale 0;
 // a gated weight's gate and up halves are padded to whole row blocks each.
 #pragma once
@@ -23,14 +24,14 @@
 
 namespace rf {
 
-constexpr int I4_ROWS = 16, I4_K = 64, I4_BLOCK = 512;
+constexpr int I4_ROWS = 16, I4_K = 64, I4_BLOCK = 512, I4_STEP = 128;
 
 struct Int4Shape {
   int64_t half_rows;   // rows of one half (N, or N / 2 gated)
   int halves;          // 2 gated, 1 otherwise
   int64_t half_blocks; // row blocks of one half
-  int64_t k_blocks;
-  int64_t groups;      // scale groups along K
+  int64_t k_blocks;    // even
+  int64_t groups;      // scale groups along K, padded to whole steps
 
   __host__ __device__ int64_t row_blocks() const { return half_blocks * halves; }
   __host__ __device__ int64_t slot_bytes() const { return row_blocks() * k_blocks * I4_BLOCK; }
@@ -42,9 +43,16 @@ inline __host__ __device__ Int4Shape int4_shape(int64_t N, int64_t K, int64_t gr
   s.halves = gated ? 2 : 1;
   s.half_rows = N / s.halves;
   s.half_blocks = (s.half_rows + I4_ROWS - 1) / I4_ROWS;
-  s.k_blocks = (K + I4_K - 1) / I4_K;
-  s.groups = (K + group - 1) / group;
+  const int64_t steps = (K + I4_STEP - 1) / I4_STEP;
+  s.k_blocks = steps * (I4_STEP / I4_K);
+  s.groups = steps * (I4_STEP / group);
   return s;
+}
+
+// Where the scale of row r16 of a row block and group gr (of subs to a step)
+// stands among the block's scales.
+inline __host__ __device__ int64_t int4_scale_at(int r16, int64_t gr, int subs) {
+  return gr / subs * (I4_ROWS * subs) + ((r16 & 7) * subs + (int)(gr % subs)) * 2 + (r16 >> 3);
 }
 
 // Sizes, group and dtype of a 4-bit weight that the kernels take.
@@ -53,19 +61,27 @@ inline bool int4_valid(int64_t N, int64_t K, int64_t group, bool gated) {
          (group == 32 || group == 64 || group == 128) && N < ((int64_t)1 << 30) && K < ((int64_t)1 << 30);
 }
 
-// The pair of codes (2 i, 2 i + 1) of a word as two 16-bit values code - 8,
+// The pair of codes (2 i, 2 i + 1) of a word as two 16-bit values code + B,
 // exact: code | 128.0 (bf16) or code | 1024.0 (fp16) has the code in its last
-// mantissa bits, and subtracting 136 or 1032 leaves code - 8.
+// mantissa bits.
+template <typename T> __device__ __forceinline__ uint32_t int4_raw(uint32_t word, int i);
+template <> __device__ __forceinline__ uint32_t int4_raw<__nv_bfloat16>(uint32_t word, int i) {
+  return ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+}
+template <> __device__ __forceinline__ uint32_t int4_raw<__half>(uint32_t word, int i) {
+  return ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+}
+// The same pair as code - 8, exact: B + 8 = 136 or 1032 less.
 template <typename T> __device__ __forceinline__ uint32_t int4_pair(uint32_t word, int i);
 template <> __device__ __forceinline__ uint32_t int4_pair<__nv_bfloat16>(uint32_t word, int i) {
-  const uint32_t b = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-  const __nv_bfloat162 off = __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));  // 136
+  const uint32_t b = int4_raw<__nv_bfloat16>(word, i);
+  const __nv_bfloat162 off = __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
   const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&b), off);
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 template <> __device__ __forceinline__ uint32_t int4_pair<__half>(uint32_t word, int i) {
-  const uint32_t b = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-  const __half2 off = __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1032
+  const uint32_t b = int4_raw<__half>(word, i);
+  const __half2 off = __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));
   const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
   return *reinterpret_cast<const uint32_t *>(&v);
 }

@@ -12,7 +12,7 @@
 // their 16 up rows) of one expert over the whole reduction, its eight warps an
 // eighth of it each; a lane's 16-byte word of the stored layout is its fragment
 // of four 16 x 16 tiles of mma.sync, the codes as exact 16-bit integers, and
-// the tokens (8 or 16 at a time) are read straight from their rows.  A group's
+// the tokens (8 at a time) are read straight from their rows.  A group's
 // sums are scaled in fp32 after its products.  The eight partial sums meet in
 // shared memory in warp order, so results do not depend on timing.  There is no
 // permutation: every block finds its expert's pairs in the ids, h and y rows
@@ -34,7 +34,7 @@ namespace {
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = FW_WARPS * 32;
 constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
-constexpr int FW_STEP = 128;    // k per step: two blocks of codes
+constexpr int FW_STEP = rf::I4_STEP;
 constexpr int KMAX = 16;
 
 struct FewArgs {
@@ -82,7 +82,7 @@ __device__ __forceinline__ float2 scale_pair(uint32_t v) {
 }
 
 struct FewShared {
-  float red[FW_WARPS][2 * 2 * 4 * 32];
+  float red[FW_WARPS][2 * 4 * 32];
   int list[FW_PAIRS];       // this expert's pairs, ascending
   uint32_t active[32];      // one bit per expert with a pair
   int expert, count, part[FW_WARPS];
@@ -145,22 +145,44 @@ __device__ __forceinline__ void find_expert(const FewArgs &p, FewShared &s, int 
 }
 
 // One step's operands in registers.
-template <int NT, int SUBS>
+template <int SUBS>
 struct FewStep {
-  uint4 q[2][2];         // [row block][block of 64 k]
+  uint4 q[2][2];      // [row block][block of 64 k]
   uint32_t s[2][SUBS];
-  uint4 x[NT][2][2];     // [8 tokens][block][half]
+  uint4 x[2][2];      // [block][half], the lane's token
 };
 
-// 32 weight rows x 8 NT tokens of the expert (from pair c0 of the list on).
+template <int SUBS>
+__device__ __forceinline__ void load_scales(const uint32_t *p, uint32_t (&s)[SUBS]) {
+  if constexpr (SUBS == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+    s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
+  } else if constexpr (SUBS == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+    s[0] = v.x, s[1] = v.y;
+  } else {
+    s[0] = __ldg(p);
+  }
+}
+
+// 32 weight rows x 8 tokens of the expert (from pair c0 of the list on).
 // SUBS: scale groups in a step's 128 k (1, 2 or 4).
-template <typename T, bool GATED, int SUBS, int NT>
+//
+// The codes go to the tensor cores as code + B (B = 128 in bf16, 1024 in fp16:
+// a shift and one three-input logic operation per pair), and a group's sums
+// start from -(B + 8) * sum x, itself a product with a matrix of ones that the
+// two row blocks share: sum x (code + B) - (B + 8) sum x = sum x (code - 8).
+// Subtracting B + 8 from every code instead took 4 of 15 instructions a word.
+// The larger terms cost at most (B + 16) * 2^-24 of |sum x| in fp32, far below
+// the 16-bit rounding of the result.
+template <typename T, bool GATED, int SUBS>
 __device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e, int unit, int c0, bool &waited) {
+  constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+  constexpr float START = std::is_same<T, __half>::value ? -1032.f : -136.f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int cnt = sm.count;
-  const int KB = (int)p.sh.k_blocks, groups = (int)p.sh.groups;
-  const int steps = (KB + 1) / 2;
+  const int steps = (int)p.sh.k_blocks / 2;
   const int st0 = steps * warp / FW_WARPS, st1 = steps * (warp + 1) / FW_WARPS;
   const uint4 *wp[2];
   const uint32_t *sp[2];
@@ -168,78 +190,82 @@ __device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e,
   for (int r = 0; r < 2; ++r) {
     int64_t rb = GATED ? unit + r * p.sh.half_blocks : 2 * (int64_t)unit + r;
     rb = (int64_t)e * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
-    wp[r] = reinterpret_cast<const uint4 *>(p.w + rb * KB * rf::I4_BLOCK) + lane;
-    sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) + rb * groups * rf::I4_ROWS) + g;
+    wp[r] = reinterpret_cast<const uint4 *>(p.w + (rb * p.sh.k_blocks + 2 * st0) * rf::I4_BLOCK) + lane;
+    sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) +
+                                               (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS) + g * SUBS;
   }
-  const T *xp[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int i = c0 + 8 * n + g;
-    const int pair = i < cnt ? sm.list[i] : -1;
-    xp[n] = pair < 0 ? nullptr : reinterpret_cast<const T *>(p.a) + (int64_t)(GATED ? pair / p.topk : pair) * p.Kd + 8 * c;
-  }
-  auto load_weights = [&](FewStep<NT, SUBS> &f, int st) {
+  // token columns past the count repeat the last one and are not stored
+  const int pair = sm.list[min(c0 + g, cnt - 1)];
+  const T *xp = reinterpret_cast<const T *>(p.a) + (int64_t)(GATED ? pair / p.topk : pair) * p.Kd + 8 * c + st0 * FW_STEP;
+  auto load_weights = [&](FewStep<SUBS> &f) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)  // codes past the last block meet zero token values
-        f.q[r][b] = ldg_stream(wp[r] + (int64_t)min(2 * st + b, KB - 1) * 32);
-#pragma unroll
-      for (int i = 0; i < SUBS; ++i) f.s[r][i] = __ldg(sp[r] + (int64_t)min(st * SUBS + i, groups - 1) * 8);
+      f.q[r][0] = ldg_stream(wp[r]);
+      f.q[r][1] = ldg_stream(wp[r] + 32);
+      load_scales<SUBS>(sp[r], f.s[r]);
+      wp[r] += 64;
+      sp[r] += 8 * SUBS;
     }
   };
-  auto load_tokens = [&](FewStep<NT, SUBS> &f, int st) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+  auto load_tokens = [&](FewStep<SUBS> &f, int st) {
+    if ((st + 1) * FW_STEP <= p.Kd) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = st * FW_STEP + 64 * b + 32 * h;
-          f.x[n][b][h] = xp[n] && k + 8 * c < p.Kd ? *reinterpret_cast<const uint4 *>(xp[n] + k) : make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int h = 0; h < 2; ++h) f.x[b][h] = *reinterpret_cast<const uint4 *>(xp + 64 * b + 32 * h);
+    } else {  // past the row's end: zeros
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          f.x[b][h] = st * FW_STEP + 64 * b + 32 * h + 8 * c < p.Kd ? *reinterpret_cast<const uint4 *>(xp + 64 * b + 32 * h)
+                                                                 : make_uint4(0u, 0u, 0u, 0u);
+    }
+    xp += FW_STEP;
   };
-  float acc[2][NT][4];
+  float acc[2][4];
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
+  auto multiply = [&](const FewStep<SUBS> &f) {
+    constexpr int PER = 4 / SUBS;  // 32-k pieces of a group
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.f;
-  auto multiply = [&](const FewStep<NT, SUBS> &f) {
+    for (int i = 0; i < SUBS; ++i) {
+      float start[4];  // - (B + 8) sum x, by token column
+      const uint32_t ones[4] = {ONES, ONES, ONES, ONES};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float d[NT][4];
+      for (int j = 0; j < PER; ++j) {
+        const uint4 xv = f.x[(i * PER + j) >> 1][(i * PER + j) & 1];
+        mma_16816<T>(start, ones, xv.x, xv.y, j == 0);
+        mma_16816<T>(start, ones, xv.z, xv.w, false);
+      }
+      const float s0 = START * start[0], s1 = START * start[1];
 #pragma unroll
-      for (int hh = 0; hh < 4; ++hh) {  // 32 k each
-        const int b = hh >> 1, h = hh & 1;
-        const uint32_t lo = h ? f.q[r][b].y : f.q[r][b].x, hi = h ? f.q[r][b].w : f.q[r][b].z;
+      for (int r = 0; r < 2; ++r) {
+        float d[4] = {s0, s1, s0, s1};
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const uint32_t fr[4] = {rf::int4_pair<T>(lo, 2 * m), rf::int4_pair<T>(hi, 2 * m),
-                                  rf::int4_pair<T>(lo, 2 * m + 1), rf::int4_pair<T>(hi, 2 * m + 1)};
-          const bool first = m == 0 && hh % (4 / SUBS) == 0;
+        for (int j = 0; j < PER; ++j) {
+          const int b = (i * PER + j) >> 1, h = (i * PER + j) & 1;
+          const uint32_t lo = h ? f.q[r][b].y : f.q[r][b].x, hi = h ? f.q[r][b].w : f.q[r][b].z;
+          const uint4 xv = f.x[b][h];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 xv = f.x[n][b][h];
-            mma_16816<T>(d[n], fr, m ? xv.z : xv.x, m ? xv.w : xv.y, first);
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t fr[4] = {rf::int4_raw<T>(lo, 2 * m), rf::int4_raw<T>(hi, 2 * m),
+                                    rf::int4_raw<T>(lo, 2 * m + 1), rf::int4_raw<T>(hi, 2 * m + 1)};
+            mma_16816<T>(d, fr, m ? xv.z : xv.x, m ? xv.w : xv.y, false);
           }
         }
-        if ((hh + 1) % (4 / SUBS) == 0) {
-          const float2 sc = scale_pair<T>(f.s[r][hh / (4 / SUBS)]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[r][n][0] = fmaf(d[n][0], sc.x, acc[r][n][0]);
-            acc[r][n][1] = fmaf(d[n][1], sc.x, acc[r][n][1]);
-            acc[r][n][2] = fmaf(d[n][2], sc.y, acc[r][n][2]);
-            acc[r][n][3] = fmaf(d[n][3], sc.y, acc[r][n][3]);
-          }
-        }
+        const float2 sc = scale_pair<T>(f.s[r][i]);
+        acc[r][0] = fmaf(d[0], sc.x, acc[r][0]);
+        acc[r][1] = fmaf(d[1], sc.x, acc[r][1]);
+        acc[r][2] = fmaf(d[2], sc.y, acc[r][2]);
+        acc[r][3] = fmaf(d[3], sc.y, acc[r][3]);
       }
     }
   };
-  FewStep<NT, SUBS> fa, fb;  // the next step is on its way while one is multiplied
-  if (st0 < st1) load_weights(fa, st0);
+  FewStep<SUBS> fa, fb;  // the next step is on its way while one is multiplied
+  if (st0 < st1) load_weights(fa);
   if (!waited) {
     wait_for_previous();  // the rows of h come from the launch before
     waited = true;
@@ -247,13 +273,13 @@ __device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e,
   if (st0 < st1) load_tokens(fa, st0);
   for (int st = st0; st < st1; st += 2) {
     if (st + 1 < st1) {
-      load_weights(fb, st + 1);
+      load_weights(fb);
       load_tokens(fb, st + 1);
     }
     multiply(fa);
     if (st + 1 >= st1) break;
     if (st + 2 < st1) {
-      load_weights(fa, st + 2);
+      load_weights(fa);
       load_tokens(fa, st + 2);
     }
     multiply(fb);
@@ -263,32 +289,28 @@ __device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e,
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sm.red[warp][((r * NT + n) * 4 + j) * 32 + lane] = acc[r][n][j];
+    for (int j = 0; j < 4; ++j) sm.red[warp][(r * 4 + j) * 32 + lane] = acc[r][j];
   __syncthreads();
   constexpr int PER = GATED ? 16 : 32;  // features of a unit
-  for (int i = threadIdx.x; i < PER * 8 * NT; i += FW_THREADS) {
-    const int f = i % PER, col = i / PER;  // feature, token of the pass
-    const int r16 = f & 15;
-    const int at = ((col >> 3) * 4 + (col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + ((col & 7) >> 1);
-    const int64_t feat = (int64_t)unit * PER + f;
-    if (c0 + col >= cnt || feat >= p.N) continue;
-    const int64_t row = sm.list[c0 + col];
-    if constexpr (GATED) {
-      float gt = 0.f, up = 0.f;
+  const int f = threadIdx.x % PER, col = threadIdx.x / PER;  // feature, token of the pass
+  const int r16 = f & 15;
+  const int at = ((col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + (col >> 1);
+  const int64_t feat = (int64_t)unit * PER + f;
+  if (col >= 8 || c0 + col >= cnt || feat >= p.N) return;
+  const int64_t row = sm.list[c0 + col];
+  if constexpr (GATED) {
+    float gt = 0.f, up = 0.f;
 #pragma unroll
-      for (int w = 0; w < FW_WARPS; ++w) {
-        gt += sm.red[w][at];
-        up += sm.red[w][at + NT * 4 * 32];
-      }
-      reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
-    } else {
-      float y = 0.f;
-#pragma unroll
-      for (int w = 0; w < FW_WARPS; ++w) y += sm.red[w][at + (f >> 4) * NT * 4 * 32];
-      reinterpret_cast<float *>(p.out)[row * p.N + feat] = y;
+    for (int w = 0; w < FW_WARPS; ++w) {
+      gt += sm.red[w][at];
+      up += sm.red[w][at + 4 * 32];
     }
+    reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
+  } else {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < FW_WARPS; ++w) y += sm.red[w][at + (f >> 4) * 4 * 32];
+    reinterpret_cast<float *>(p.out)[row * p.N + feat] = y;
   }
 }
 
@@ -302,7 +324,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
   bool waited = GATED;
   const int cnt = sm.count;
   for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-    for (int c0 = 0; c0 < cnt; c0 += 8) few_pass<T, GATED, SUBS, 1>(p, sm, e, unit, c0, waited);
+    for (int c0 = 0; c0 < cnt; c0 += 8) few_pass<T, GATED, SUBS>(p, sm, e, unit, c0, waited);
   }
 }
 

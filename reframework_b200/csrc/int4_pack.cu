@@ -73,18 +73,20 @@ __global__ void __launch_bounds__(THREADS) int4_pack_kernel(const PackArgs a) {
   }
 }
 
-// One thread per (slot, row block, group, entry).
+// One thread per (slot, row block, group, row).
 template <typename T>
 __global__ void __launch_bounds__(THREADS) int4_scales_kernel(const PackArgs a) {
   const int64_t n = a.S * a.sh.slot_scales();
   for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
-    const int entry = (int)(i % rf::I4_ROWS);
+    const int r16 = (int)(i % rf::I4_ROWS);
     const int64_t g = i / rf::I4_ROWS % a.sh.groups;
     const int64_t rbs = i / rf::I4_ROWS / a.sh.groups;
     const int64_t rb = rbs % a.sh.row_blocks(), s = rbs / a.sh.row_blocks();
-    const int64_t row = source_row(a.sh, rb, (entry >> 1) + 8 * (entry & 1));
-    reinterpret_cast<T *>(a.scales)[i] =
-        row >= 0 ? reinterpret_cast<const T *>(a.scales_in)[(s * a.N + row) * a.sh.groups + g] : rf::Cvt<T>::from_f(0.f);
+    const int64_t row = source_row(a.sh, rb, r16);
+    const int64_t groups = (a.K + a.group - 1) / a.group;
+    reinterpret_cast<T *>(a.scales)[rbs * a.sh.groups * rf::I4_ROWS + rf::int4_scale_at(r16, g, rf::I4_STEP / a.group)] =
+        row >= 0 && g < groups ? reinterpret_cast<const T *>(a.scales_in)[(s * a.N + row) * groups + g]
+                               : rf::Cvt<T>::from_f(0.f);
   }
 }
 
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(THREADS) int4_quantize_kernel(const PackArgs a
         code[r16][lane + 32 * i] = (uint8_t)((int)q + 8);
         const int64_t g = (k0 + 32 * i) / a.group;
         if (lane == 0 && (32 * i) % a.group == 0 && g < a.sh.groups)
-          scales[g * rf::I4_ROWS + 2 * (r16 & 7) + (r16 >> 3)] = rf::Cvt<T>::from_f(row >= 0 ? sc : 0.f);
+          scales[rf::int4_scale_at(r16, g, rf::I4_STEP / a.group)] = rf::Cvt<T>::from_f(row >= 0 ? sc : 0.f);
       }
     }
     __syncthreads();
@@ -176,7 +178,8 @@ __global__ void __launch_bounds__(THREADS) int4_dequantize_kernel(const PackArgs
         const uint32_t w = word[2 * h + (j >> 3)];
         const int code = (int)(w >> (4 * ((j & 7) / 2 + 4 * (j & 1))) & 15u);
         const float sc = rf::Cvt<T>::to_f(
-            reinterpret_cast<const T *>(a.scales)[(rbs * a.sh.groups + k / a.group) * rf::I4_ROWS + 2 * (lane >> 2) + h]);
+            reinterpret_cast<const T *>(a.scales)[rbs * a.sh.groups * rf::I4_ROWS +
+                                                  rf::int4_scale_at((lane >> 2) + 8 * h, k / a.group, rf::I4_STEP / a.group)]);
         reinterpret_cast<T *>(a.out)[(s * a.N + row) * a.K + k] = rf::Cvt<T>::from_f(sc * (float)(code - 8));
       }
     }

@@ -473,11 +473,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         const int at = GATED ? 4 * r + j : 2 * j + r;
         const uint32_t src = codes + (uint32_t)(at * Q_KSUB * rf::I4_BLOCK + lane * 16);
         const uint32_t ss = codes + Q_CODE_BYTES +
-                            (uint32_t)((at >> 2) * (Q_SCALE_BYTES / 2) + (at & 3) * (SUBS * rf::I4_ROWS * 2) + g * 4);
+                            (uint32_t)((at >> 2) * (Q_SCALE_BYTES / 2) + (at & 3) * (SUBS * rf::I4_ROWS * 2) + g * SUBS * 4);
 #pragma unroll
         for (int b = 0; b < Q_KSUB; ++b) q[r][b] = ld_shared_v4(src + (uint32_t)(b * rf::I4_BLOCK));
 #pragma unroll
-        for (int i = 0; i < SUBS; ++i) sc[r][i] = ld_shared_u32(ss + (uint32_t)(i * rf::I4_ROWS * 2));
+        for (int i = 0; i < SUBS; ++i) sc[r][i] = ld_shared_u32(ss + (uint32_t)(i * 4));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(CEMPTY(slot));  // the codes are in registers
@@ -601,7 +601,7 @@ int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st) {
   p.group = g.group;
   p.act = g.act;
   p.sh = int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated);
-  // codes as [E * row blocks][k blocks * 128] words, scales as [E * row blocks][groups * 16]
+  // codes as [E * row blocks][k blocks * 128] words, scales as [E * row blocks][padded groups * 16]
   const uint64_t rows = (uint64_t)g.E * (uint64_t)p.sh.row_blocks();
   const uint32_t scale_cols = (uint32_t)(Q_KSUB * Q_BK / g.group * rf::I4_ROWS);
   CUtensorMap mw, ms;

@@ -21,6 +21,7 @@
 // rows only after its ids and first weights are on the way.
 // Many rows per expert: permute with the row gather, then int4_pair.cu.
 #include <algorithm>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -35,6 +36,7 @@ constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = FW_WARPS * 32;
 constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
 constexpr int FW_STEP = rf::I4_STEP;
+constexpr int FW_AHEAD = 4;     // ring slots of a warp: steps of codes on their way, and the one in use
 constexpr int KMAX = 16;
 
 struct FewArgs {
@@ -82,90 +84,92 @@ __device__ __forceinline__ float2 scale_pair(uint32_t v) {
 }
 
 struct FewShared {
+  uint4 ring[FW_WARPS][FW_AHEAD][4][32];   // codes on their way, by lane
+  uint32_t scale[FW_WARPS][FW_AHEAD][2][32];  // and their scales (8 rows x up to 4 groups)
   float red[FW_WARPS][2 * 4 * 32];
-  int list[FW_PAIRS];       // this expert's pairs, ascending
-  uint32_t active[32];      // one bit per expert with a pair
-  int expert, count, part[FW_WARPS];
+  int count[1024];          // pairs of each expert
+  int prefix[1025];         // passes (8 pairs each) before the y-th expert that has pairs
+  int list[FW_PAIRS];       // the current expert's pairs, ascending
+  uint16_t expert[1024];    // the experts that have pairs, ascending
+  int active, part[FW_WARPS];
 };
 
-// The y-th expert (ascending) that some pair names, its pairs into s.list and
-// their number; expert -1 if there are not so many.
-__device__ __forceinline__ void find_expert(const FewArgs &p, FewShared &s, int y, bool report) {
+// A job is 32 weight rows of one expert against 8 of its tokens; a launch's jobs
+// in the order expert, unit (of 32 rows), pass (of 8 tokens).
+struct FewJob {
+  int y, unit, pass;
+};
+
+// Counts each expert's pairs; the experts that have any, with their passes summed up.
+__device__ __forceinline__ void count_experts(const FewArgs &p, FewShared &s, const int (&id)[FW_PAIRS / FW_THREADS]) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < 32) s.active[tid] = 0u;
-  if (tid == 0) s.count = 0;
-  int id[FW_PAIRS / FW_THREADS];
-#pragma unroll
-  for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i) {
-    const int at = i * FW_THREADS + tid;
-    id[i] = at < p.pairs ? p.ids[at] : -1;
-    if (at < p.pairs && (unsigned)id[i] >= (unsigned)p.E) {
-      if (report) rf_report(RF_DEV_BAD_EXPERT_ID);
-      id[i] = -1;
-    }
-  }
+  for (int e = tid; e < p.E; e += FW_THREADS) s.count[e] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i)
-    if (id[i] >= 0) atomicOr(&s.active[id[i] >> 5], 1u << (id[i] & 31));
+    if (id[i] >= 0) atomicAdd(&s.count[id[i]], 1);
   __syncthreads();
   if (warp == 0) {
-    const uint32_t bits = s.active[lane];
-    const int n = __popc(bits);
-    int before = n;
+    int n = 0, passes = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int cnt = e0 + lane < p.E ? s.count[e0 + lane] : 0;
+      const unsigned b = __ballot_sync(0xffffffffu, cnt > 0);
+      const int mine = (cnt + 7) / 8;
+      int upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      if (cnt > 0) {
+        const int y = n + __popc(b & ((1u << lane) - 1u));
+        s.expert[y] = (uint16_t)(e0 + lane);
+        s.prefix[y] = passes + upto - mine;
+      }
+      n += __popc(b);
+      passes += __shfl_sync(0xffffffffu, upto, 31);
     }
-    before -= n;
-    if (lane == 31 && y >= before + n) s.expert = -1;
-    if (y >= before && y < before + n) s.expert = lane * 32 + (int)__fns(bits, 0, y - before + 1);
+    if (lane == 0) {
+      s.active = n;
+      s.prefix[n] = passes;
+    }
   }
   __syncthreads();
-  const int e = s.expert;
-  if (e < 0) return;
+}
+
+// The pairs of expert e, ascending, into s.list.
+__device__ __forceinline__ void list_pairs(const FewArgs &p, FewShared &s, const int (&id)[FW_PAIRS / FW_THREADS], int e) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int base = 0;
+  __syncthreads();  // the previous expert's list has been read
 #pragma unroll
   for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i) {
     if (i * FW_THREADS >= p.pairs) break;
     const unsigned b = __ballot_sync(0xffffffffu, id[i] == e);
     if (lane == 0) s.part[warp] = __popc(b);
     __syncthreads();
-    int base = s.count, all = 0;
+    int at = base;
 #pragma unroll
     for (int w = 0; w < FW_WARPS; ++w) {
-      base += w < warp ? s.part[w] : 0;
-      all += s.part[w];
+      at += w < warp ? s.part[w] : 0;
+      base += s.part[w];
     }
-    if (id[i] == e) s.list[base + __popc(b & ((1u << lane) - 1u))] = i * FW_THREADS + tid;
+    if (id[i] == e) s.list[at + __popc(b & ((1u << lane) - 1u))] = i * FW_THREADS + tid;
     __syncthreads();
-    if (tid == 0) s.count += all;
-  }
-  __syncthreads();
-}
-
-// One step's operands in registers.
-template <int SUBS>
-struct FewStep {
-  uint4 q[2][2];      // [row block][block of 64 k]
-  uint32_t s[2][SUBS];
-  uint4 x[2][2];      // [block][half], the lane's token
-};
-
-template <int SUBS>
-__device__ __forceinline__ void load_scales(const uint32_t *p, uint32_t (&s)[SUBS]) {
-  if constexpr (SUBS == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-    s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
-  } else if constexpr (SUBS == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-    s[0] = v.x, s[1] = v.y;
-  } else {
-    s[0] = __ldg(p);
   }
 }
 
-// 32 weight rows x 8 tokens of the expert (from pair c0 of the list on).
+__device__ __forceinline__ void copy16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_small(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
 // SUBS: scale groups in a step's 128 k (1, 2 or 4).
 //
 // The codes go to the tensor cores as code + B (B = 128 in bf16, 1024 in fp16:
@@ -175,167 +179,222 @@ __device__ __forceinline__ void load_scales(const uint32_t *p, uint32_t (&s)[SUB
 // Subtracting B + 8 from every code instead took 4 of 15 instructions a word.
 // The larger terms cost at most (B + 16) * 2^-24 of |sum x| in fp32, far below
 // the 16-bit rounding of the result.
+//
+// Each warp copies its codes into a ring of its own, FW_AHEAD - 1 steps before
+// their use and across the ends of jobs: a job is only a few steps long per
+// warp (4 at K = 4096), and the memory would idle at each end.
 template <typename T, bool GATED, int SUBS>
-__device__ __forceinline__ void few_pass(const FewArgs &p, FewShared &sm, int e, int unit, int c0, bool &waited) {
+__global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
+  extern __shared__ __align__(16) uint8_t few_smem[];
+  FewShared &sm = *reinterpret_cast<FewShared *>(few_smem);
   constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
   constexpr float START = std::is_same<T, __half>::value ? -1032.f : -136.f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int cnt = sm.count;
+  launch_dependents();
+  int id[FW_PAIRS / FW_THREADS];  // this thread's pairs' experts
+#pragma unroll
+  for (int i = 0; i < FW_PAIRS / FW_THREADS; ++i) {
+    const int at = i * FW_THREADS + (int)threadIdx.x;
+    id[i] = at < p.pairs ? p.ids[at] : -1;
+    if (at < p.pairs && (unsigned)id[i] >= (unsigned)p.E) {
+      if (GATED && blockIdx.x == 0) rf_report(RF_DEV_BAD_EXPERT_ID);
+      id[i] = -1;
+    }
+  }
+  count_experts(p, sm, id);
+  const int n = sm.active;
+  const int64_t jobs = (int64_t)sm.prefix[n] * p.units;
+  const int j0 = (int)(jobs * blockIdx.x / gridDim.x), j1 = (int)(jobs * (blockIdx.x + 1) / gridDim.x);
+  if (j0 >= j1) return;
   const int steps = (int)p.sh.k_blocks / 2;
-  const int st0 = steps * warp / FW_WARPS, st1 = steps * (warp + 1) / FW_WARPS;
+  const int st0 = steps * warp / FW_WARPS, mine = steps * (warp + 1) / FW_WARPS - st0;  // this warp's steps of a job
+
+  auto passes_of = [&](int y) { return sm.prefix[y + 1] - sm.prefix[y]; };
+  auto job_at = [&](int j) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)sm.prefix[mid] * p.units <= j) lo = mid;
+      else hi = mid - 1;
+    }
+    const int at = j - sm.prefix[lo] * p.units, np = passes_of(lo);
+    return FewJob{lo, at / np, at % np};
+  };
+  auto next_job = [&](FewJob &b) {
+    if (++b.pass < passes_of(b.y)) return;
+    b.pass = 0;
+    if (++b.unit < p.units) return;
+    b.unit = 0;
+    ++b.y;
+  };
+
+  // ---- the copy cursor: step cst of job cj, for this lane
+  FewJob cb = job_at(j0);
+  int cj = j0, cst = 0, cslot = 0;
   const uint4 *wp[2];
   const uint32_t *sp[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    int64_t rb = GATED ? unit + r * p.sh.half_blocks : 2 * (int64_t)unit + r;
-    rb = (int64_t)e * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
-    wp[r] = reinterpret_cast<const uint4 *>(p.w + (rb * p.sh.k_blocks + 2 * st0) * rf::I4_BLOCK) + lane;
-    sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) +
-                                               (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS) + g * SUBS;
-  }
-  // token columns past the count repeat the last one and are not stored
-  const int pair = sm.list[min(c0 + g, cnt - 1)];
-  const T *xp = reinterpret_cast<const T *>(p.a) + (int64_t)(GATED ? pair / p.topk : pair) * p.Kd + 8 * c + st0 * FW_STEP;
-  auto load_weights = [&](FewStep<SUBS> &f) {
+  auto open_job = [&]() {
+    if (cj >= j1) return;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      f.q[r][0] = ldg_stream(wp[r]);
-      f.q[r][1] = ldg_stream(wp[r] + 32);
-      load_scales<SUBS>(sp[r], f.s[r]);
-      wp[r] += 64;
-      sp[r] += 8 * SUBS;
+      int64_t rb = GATED ? cb.unit + r * p.sh.half_blocks : 2 * (int64_t)cb.unit + r;
+      rb = (int64_t)sm.expert[cb.y] * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
+      wp[r] = reinterpret_cast<const uint4 *>(p.w + (rb * p.sh.k_blocks + 2 * st0) * rf::I4_BLOCK) + lane;
+      sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) +
+                                                 (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS);
     }
   };
-  auto load_tokens = [&](FewStep<SUBS> &f, int st) {
-    if ((st + 1) * FW_STEP <= p.Kd) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) f.x[b][h] = *reinterpret_cast<const uint4 *>(xp + 64 * b + 32 * h);
-    } else {  // past the row's end: zeros
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          f.x[b][h] = st * FW_STEP + 64 * b + 32 * h + 8 * c < p.Kd ? *reinterpret_cast<const uint4 *>(xp + 64 * b + 32 * h)
-                                                                 : make_uint4(0u, 0u, 0u, 0u);
-    }
-    xp += FW_STEP;
-  };
-  float acc[2][4];
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
-  auto multiply = [&](const FewStep<SUBS> &f) {
-    constexpr int PER = 4 / SUBS;  // 32-k pieces of a group
-#pragma unroll
-    for (int i = 0; i < SUBS; ++i) {
-      float start[4];  // - (B + 8) sum x, by token column
-      const uint32_t ones[4] = {ONES, ONES, ONES, ONES};
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const uint4 xv = f.x[(i * PER + j) >> 1][(i * PER + j) & 1];
-        mma_16816<T>(start, ones, xv.x, xv.y, j == 0);
-        mma_16816<T>(start, ones, xv.z, xv.w, false);
-      }
-      const float s0 = START * start[0], s1 = START * start[1];
+  auto copy_step = [&]() {
+    if (cj < j1) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float d[4] = {s0, s1, s0, s1};
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int b = (i * PER + j) >> 1, h = (i * PER + j) & 1;
-          const uint32_t lo = h ? f.q[r][b].y : f.q[r][b].x, hi = h ? f.q[r][b].w : f.q[r][b].z;
-          const uint4 xv = f.x[b][h];
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint32_t fr[4] = {rf::int4_raw<T>(lo, 2 * m), rf::int4_raw<T>(hi, 2 * m),
-                                    rf::int4_raw<T>(lo, 2 * m + 1), rf::int4_raw<T>(hi, 2 * m + 1)};
-            mma_16816<T>(d, fr, m ? xv.z : xv.x, m ? xv.w : xv.y, false);
-          }
-        }
-        const float2 sc = scale_pair<T>(f.s[r][i]);
-        acc[r][0] = fmaf(d[0], sc.x, acc[r][0]);
-        acc[r][1] = fmaf(d[1], sc.x, acc[r][1]);
-        acc[r][2] = fmaf(d[2], sc.y, acc[r][2]);
-        acc[r][3] = fmaf(d[3], sc.y, acc[r][3]);
+        copy16(&sm.ring[warp][cslot][2 * r][lane], wp[r]);
+        copy16(&sm.ring[warp][cslot][2 * r + 1][lane], wp[r] + 32);
+        // 8 SUBS words of a row block: each lane copies the words that it will read
+        if (SUBS == 4) { if (c == 0) copy16(&sm.scale[warp][cslot][r][g * 4], sp[r] + g * 4); }
+        else if (c == 0) copy_small<4 * SUBS>(&sm.scale[warp][cslot][r][g * SUBS], sp[r] + g * SUBS);
+        wp[r] += 64;
+        sp[r] += 8 * SUBS;
+      }
+      if (++cst == mine) {
+        cst = 0;
+        ++cj;
+        next_job(cb);
+        open_job();
       }
     }
+    copies_commit();
+    cslot = cslot + 1 == FW_AHEAD ? 0 : cslot + 1;
   };
-  FewStep<SUBS> fa, fb;  // the next step is on its way while one is multiplied
-  if (st0 < st1) load_weights(fa);
-  if (!waited) {
-    wait_for_previous();  // the rows of h come from the launch before
-    waited = true;
+  if (mine > 0) {
+    open_job();
+    for (int i = 0; i < FW_AHEAD - 1; ++i) copy_step();
   }
-  if (st0 < st1) load_tokens(fa, st0);
-  for (int st = st0; st < st1; st += 2) {
-    if (st + 1 < st1) {
-      load_weights(fb);
-      load_tokens(fb, st + 1);
-    }
-    multiply(fa);
-    if (st + 1 >= st1) break;
-    if (st + 2 < st1) {
-      load_weights(fa);
-      load_tokens(fa, st + 2);
-    }
-    multiply(fb);
-  }
-  // ---- the warps' partial sums, in warp order
-  __syncthreads();  // the previous pass's sums have been read
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sm.red[warp][(r * 4 + j) * 32 + lane] = acc[r][j];
-  __syncthreads();
-  constexpr int PER = GATED ? 16 : 32;  // features of a unit
-  const int f = threadIdx.x % PER, col = threadIdx.x / PER;  // feature, token of the pass
-  const int r16 = f & 15;
-  const int at = ((col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + (col >> 1);
-  const int64_t feat = (int64_t)unit * PER + f;
-  if (col >= 8 || c0 + col >= cnt || feat >= p.N) return;
-  const int64_t row = sm.list[c0 + col];
-  if constexpr (GATED) {
-    float gt = 0.f, up = 0.f;
-#pragma unroll
-    for (int w = 0; w < FW_WARPS; ++w) {
-      gt += sm.red[w][at];
-      up += sm.red[w][at + 4 * 32];
-    }
-    reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
-  } else {
-    float y = 0.f;
-#pragma unroll
-    for (int w = 0; w < FW_WARPS; ++w) y += sm.red[w][at + (f >> 4) * 4 * 32];
-    reinterpret_cast<float *>(p.out)[row * p.N + feat] = y;
-  }
-}
+  if (!GATED) wait_for_previous();  // the rows of h come from the launch before
 
-template <typename T, bool GATED, int SUBS>
-__global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
-  __shared__ FewShared sm;
-  launch_dependents();
-  find_expert(p, sm, blockIdx.y, GATED && blockIdx.x == 0 && blockIdx.y == 0);
-  const int e = sm.expert;
-  if (e < 0) return;
-  bool waited = GATED;
-  const int cnt = sm.count;
-  for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-    for (int c0 = 0; c0 < cnt; c0 += 8) few_pass<T, GATED, SUBS>(p, sm, e, unit, c0, waited);
+  FewJob b = job_at(j0);
+  int y = -1, cnt = 0, slot = 0;
+  for (int j = j0; j < j1; ++j, next_job(b)) {
+    if (b.y != y) {
+      y = b.y;
+      cnt = sm.count[sm.expert[y]];
+      list_pairs(p, sm, id, sm.expert[y]);
+    }
+    const int c0 = 8 * b.pass;
+    // token columns past the count repeat the last one and are not stored
+    const int pair = sm.list[min(c0 + g, cnt - 1)];
+    const T *xp = reinterpret_cast<const T *>(p.a) + (int64_t)(GATED ? pair / p.topk : pair) * p.Kd + 8 * c;
+    uint4 x[2][2];
+    auto load_tokens = [&](int st) {
+      const T *q = xp + st * FW_STEP;
+      if ((st + 1) * FW_STEP <= p.Kd) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k >> 1][k & 1] = *reinterpret_cast<const uint4 *>(q + 32 * k);
+      } else {  // past the row's end: zeros
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k >> 1][k & 1] = st * FW_STEP + 32 * k + 8 * c < p.Kd ? *reinterpret_cast<const uint4 *>(q + 32 * k)
+                                                               : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    float acc[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[r][i] = 0.f;
+    for (int s = 0; s < mine; ++s) {
+      load_tokens(st0 + s);
+      copies_wait<FW_AHEAD - 2>();
+      __syncwarp();  // a lane's scales were copied by another one
+      copy_step();
+      constexpr int PER = 4 / SUBS;  // 32-k pieces of a group
+      uint4 q[2][2];
+      uint32_t sc[2][SUBS];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        q[r][0] = sm.ring[warp][slot][2 * r][lane];
+        q[r][1] = sm.ring[warp][slot][2 * r + 1][lane];
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) sc[r][i] = sm.scale[warp][slot][r][g * SUBS + i];
+      }
+      slot = slot + 1 == FW_AHEAD ? 0 : slot + 1;
+#pragma unroll
+      for (int i = 0; i < SUBS; ++i) {
+        float start[4];  // - (B + 8) sum x, by token column
+        const uint32_t ones[4] = {ONES, ONES, ONES, ONES};
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const uint4 xv = x[(i * PER + k) >> 1][(i * PER + k) & 1];
+          mma_16816<T>(start, ones, xv.x, xv.y, k == 0);
+          mma_16816<T>(start, ones, xv.z, xv.w, false);
+        }
+        const float s0 = START * start[0], s1 = START * start[1];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float d[4] = {s0, s1, s0, s1};
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const int bl = (i * PER + k) >> 1, h = (i * PER + k) & 1;
+            const uint32_t lo = h ? q[r][bl].y : q[r][bl].x, hi = h ? q[r][bl].w : q[r][bl].z;
+            const uint4 xv = x[bl][h];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const uint32_t fr[4] = {rf::int4_raw<T>(lo, 2 * m), rf::int4_raw<T>(hi, 2 * m),
+                                      rf::int4_raw<T>(lo, 2 * m + 1), rf::int4_raw<T>(hi, 2 * m + 1)};
+              mma_16816<T>(d, fr, m ? xv.z : xv.x, m ? xv.w : xv.y, false);
+            }
+          }
+          const float2 f = scale_pair<T>(sc[r][i]);
+          acc[r][0] = fmaf(d[0], f.x, acc[r][0]);
+          acc[r][1] = fmaf(d[1], f.x, acc[r][1]);
+          acc[r][2] = fmaf(d[2], f.y, acc[r][2]);
+          acc[r][3] = fmaf(d[3], f.y, acc[r][3]);
+        }
+      }
+    }
+    // ---- the warps' partial sums, in warp order
+    __syncthreads();  // the previous job's sums have been read
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sm.red[warp][(r * 4 + i) * 32 + lane] = acc[r][i];
+    __syncthreads();
+    constexpr int PER = GATED ? 16 : 32;  // features of a unit
+    const int f = threadIdx.x % PER, col = threadIdx.x / PER;  // feature, token of the job
+    const int r16 = f & 15;
+    const int at = ((col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + (col >> 1);
+    const int64_t feat = (int64_t)b.unit * PER + f;
+    if (col < 8 && c0 + col < cnt && feat < p.N) {
+      const int64_t row = sm.list[c0 + col];
+      if constexpr (GATED) {
+        float gt = 0.f, up = 0.f;
+#pragma unroll
+        for (int w = 0; w < FW_WARPS; ++w) {
+          gt += sm.red[w][at];
+          up += sm.red[w][at + 4 * 32];
+        }
+        reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
+      } else {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < FW_WARPS; ++w) v += sm.red[w][at + (f >> 4) * 4 * 32];
+        reinterpret_cast<float *>(p.out)[row * p.N + feat] = v;
+      }
+    }
   }
+  copies_wait<0>();
 }
 
 // Launches `kern` so that it may start while the previous launch on the stream
 // drains (it waits for it itself, wait_for_previous).
 template <typename... Params, typename... Args>
-int launch_chained(const char *what, void (*kern)(Params...), dim3 grid, int threads, bool chained, cudaStream_t st,
-                   Args... args) {
+int launch_chained(const char *what, void (*kern)(Params...), dim3 grid, int threads, size_t smem, bool chained,
+                   cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -350,24 +409,40 @@ int launch_chained(const char *what, void (*kern)(Params...), dim3 grid, int thr
   return RF_OK;
 }
 
-template <typename T, bool GATED>
-int launch_few_t(const FewArgs &p, int group, dim3 grid, cudaStream_t st) {
+template <typename T, bool GATED, int SUBS>
+int launch_few_s(const FewArgs &p, cudaStream_t st) {
+  auto kern = int4_few_kernel<T, GATED, SUBS>;
   const char *what = GATED ? "4-bit gated products (few rows)" : "4-bit down products (few rows)";
-  if (group == 32) return launch_chained(what, int4_few_kernel<T, GATED, 4>, grid, FW_THREADS, !GATED, st, p);
-  if (group == 64) return launch_chained(what, int4_few_kernel<T, GATED, 2>, grid, FW_THREADS, !GATED, st, p);
-  return launch_chained(what, int4_few_kernel<T, GATED, 1>, grid, FW_THREADS, !GATED, st, p);
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  static int resident = 0;
+  std::call_once(once, [&] {
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FewShared));
+    if (err == cudaSuccess) err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, FW_THREADS, sizeof(FewShared));
+  });
+  if (err != cudaSuccess || resident < 1) {
+    cudaGetLastError();
+    return rf::fail(RF_ERR_CUDA, std::string(what) + ": the kernel does not fit this device");
+  }
+  // as many blocks as run at once share the jobs (at most units * pairs) evenly
+  const int64_t most = (int64_t)p.units * p.pairs;
+  const int64_t blocks = std::min<int64_t>(most, (int64_t)rf::num_sms() * resident);
+  return launch_chained(what, kern, dim3((unsigned)blocks), FW_THREADS, sizeof(FewShared), !GATED, st, p);
+}
+
+template <typename T, bool GATED>
+int launch_few_t(const FewArgs &p, int group, cudaStream_t st) {
+  if (group == 32) return launch_few_s<T, GATED, 4>(p, st);
+  if (group == 64) return launch_few_s<T, GATED, 2>(p, st);
+  return launch_few_s<T, GATED, 1>(p, st);
 }
 
 int launch_few(const rf::Int4Gemm &g, bool gated, const int32_t *ids, int topk, cudaStream_t st) {
   const rf::Int4Shape sh = rf::int4_shape(gated ? 2 * (int64_t)g.N : g.N, g.Kdim, g.group, gated);
   const int units = (int)(gated ? sh.half_blocks : (sh.row_blocks() + 1) / 2);
   const FewArgs p{g.a, g.w, g.scales, g.out, ids, (int)g.rows, topk, g.E, g.N, g.Kdim, g.act, units, sh};
-  // a block per unit and expert, fewer where that is more than eight waves
-  const int active = (int)std::min<int64_t>(g.E, g.rows);
-  const int most = std::max(1, rf::num_sms() * 16 / active);
-  const dim3 grid((unsigned)std::min(units, most), (unsigned)active);
-  if (g.dtype == RF_F16) return gated ? launch_few_t<__half, true>(p, g.group, grid, st) : launch_few_t<__half, false>(p, g.group, grid, st);
-  return gated ? launch_few_t<__nv_bfloat16, true>(p, g.group, grid, st) : launch_few_t<__nv_bfloat16, false>(p, g.group, grid, st);
+  if (g.dtype == RF_F16) return gated ? launch_few_t<__half, true>(p, g.group, st) : launch_few_t<__half, false>(p, g.group, st);
+  return gated ? launch_few_t<__nv_bfloat16, true>(p, g.group, st) : launch_few_t<__nv_bfloat16, false>(p, g.group, st);
 }
 
 // ------------------------------------------------------------------ combine
@@ -432,7 +507,7 @@ template <typename T>
 int launch_combine(const CombineArgs &a, cudaStream_t st) {
   const int64_t gy = (a.H + CB_THREADS * 8 - 1) / (CB_THREADS * 8);
   const int64_t gx = std::min<int64_t>(a.T, std::max<int64_t>(1, (int64_t)rf::num_sms() * 16 / gy));
-  return launch_chained("4-bit combine", int4_combine_kernel<T>, dim3((unsigned)gx, (unsigned)gy), CB_THREADS, a.ids != nullptr,
+  return launch_chained("4-bit combine", int4_combine_kernel<T>, dim3((unsigned)gx, (unsigned)gy), CB_THREADS, 0, a.ids != nullptr,
                         st, a);
 }
 
@@ -468,7 +543,7 @@ Layout make_layout(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
 
 bool sizes_ok(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
   return T >= 0 && K >= 1 && K <= KMAX && E >= 1 && E <= 1024 && H > 0 && I > 0 && H % 8 == 0 && I % 8 == 0 &&
-         H < ((int64_t)1 << 28) && I < ((int64_t)1 << 28) && T <= 0x7fffffff / K;
+         H <= ((int64_t)1 << 20) && I <= ((int64_t)1 << 20) && T <= 0x7fffffff / K;
 }
 
 // The CTA-pair kernel from this many rows per expert on (the mean over the
@@ -498,7 +573,7 @@ extern "C" int rf_moe_int4_experts(const void *x, int dtype, const void *w1, con
   RF_CHECK_ARG(dtype == RF_F16 || dtype == RF_BF16, "rf_moe_int4_experts: 4-bit experts serve bf16 and fp16 layers");
   RF_CHECK_ARG(activation >= RF_ACT_SILU && activation <= RF_ACT_GELU_TANH, "rf_moe_int4_experts: unknown activation");
   RF_CHECK_ARG(sizes_ok(T, K, E, H, I),
-               "rf_moe_int4_experts: bad sizes (K <= 16, E <= 1024, H and I multiples of 8, T * K < 2^31)");
+               "rf_moe_int4_experts: bad sizes (K <= 16, E <= 1024, H and I multiples of 8 up to 2^20, T * K < 2^31)");
   RF_CHECK_ARG(rf::int4_valid(2 * I, H, w1_group, true) && rf::int4_valid(H, I, w2_group, false),
                "rf_moe_int4_experts: group sizes must be 32, 64 or 128");
   RF_CHECK_ARG(w1 && w1_scales && w2 && w2_scales, "rf_moe_int4_experts: null weights");

@@ -36,7 +36,7 @@ constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = FW_WARPS * 32;
 constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
 constexpr int FW_STEP = rf::I4_STEP;
-constexpr int FW_AHEAD = 4;     // ring slots of a warp: steps of codes on their way, and the one in use
+constexpr int FW_AHEAD = 4;     // a power of two: ring slots of a warp: steps of codes on their way, and the one in use
 constexpr int KMAX = 16;
 
 struct FewArgs {
@@ -49,29 +49,22 @@ struct FewArgs {
   rf::Int4Shape sh;
 };
 
-// d = a . b + (first ? 0 : d)
+// d = a . b + c, c four registers or zeros
 template <typename T>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
-  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                          const float (&c)[4]) {
   if constexpr (std::is_same<T, __half>::value)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {  // weights pass through once: not kept in L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Waits until the launch before this one is complete and its writes visible.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -159,13 +152,11 @@ __device__ __forceinline__ void list_pairs(const FewArgs &p, FewShared &s, const
   }
 }
 
-__device__ __forceinline__ void copy16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
+// Bytes to shared address dst; 16 bypass L1.
 template <int BYTES>
-__device__ __forceinline__ void copy_small(void *dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES)
-               : "memory");
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void *src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -174,8 +165,8 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile
 //
 // The codes go to the tensor cores as code + B (B = 128 in bf16, 1024 in fp16:
 // a shift and one three-input logic operation per pair), and a group's sums
-// start from -(B + 8) * sum x, itself a product with a matrix of ones that the
-// two row blocks share: sum x (code + B) - (B + 8) sum x = sum x (code - 8).
+// start from -(B + 8) * sum x, itself a product, with a matrix of -(B + 8), that
+// the two row blocks share: sum x (code + B) - (B + 8) sum x = sum x (code - 8).
 // Subtracting B + 8 from every code instead took 4 of 15 instructions a word.
 // The larger terms cost at most (B + 16) * 2^-24 of |sum x| in fp32, far below
 // the 16-bit rounding of the result.
@@ -187,8 +178,7 @@ template <typename T, bool GATED, int SUBS>
 __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
   extern __shared__ __align__(16) uint8_t few_smem[];
   FewShared &sm = *reinterpret_cast<FewShared *>(few_smem);
-  constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
-  constexpr float START = std::is_same<T, __half>::value ? -1032.f : -136.f;
+  constexpr uint32_t OFFSET = std::is_same<T, __half>::value ? 0xe408e408u : 0xc308c308u;  // -1032, -136 twice
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   launch_dependents();
@@ -242,18 +232,19 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
       rb = (int64_t)sm.expert[cb.y] * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
       wp[r] = reinterpret_cast<const uint4 *>(p.w + (rb * p.sh.k_blocks + 2 * st0) * rf::I4_BLOCK) + lane;
       sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) +
-                                                 (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS);
+                                                 (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS) + g * SUBS;
     }
   };
+  const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(&sm.ring[warp][0][0][lane]);
+  const uint32_t scale0 = (uint32_t)__cvta_generic_to_shared(&sm.scale[warp][0][0][g * SUBS]);
   auto copy_step = [&]() {
     if (cj < j1) {
+      const uint32_t rd = ring0 + (uint32_t)cslot * (4 * 32 * 16), sd = scale0 + (uint32_t)cslot * (2 * 32 * 4);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        copy16(&sm.ring[warp][cslot][2 * r][lane], wp[r]);
-        copy16(&sm.ring[warp][cslot][2 * r + 1][lane], wp[r] + 32);
-        // 8 SUBS words of a row block: each lane copies the words that it will read
-        if (SUBS == 4) { if (c == 0) copy16(&sm.scale[warp][cslot][r][g * 4], sp[r] + g * 4); }
-        else if (c == 0) copy_small<4 * SUBS>(&sm.scale[warp][cslot][r][g * SUBS], sp[r] + g * SUBS);
+        copy_bytes<16>(rd + (2 * r) * 512, wp[r]);
+        copy_bytes<16>(rd + (2 * r + 1) * 512, wp[r] + 32);
+        if (c == 0) copy_bytes<4 * SUBS>(sd + r * 128, sp[r]);  // its row's scales, for the row's four lanes
         wp[r] += 64;
         sp[r] += 8 * SUBS;
       }
@@ -265,7 +256,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
       }
     }
     copies_commit();
-    cslot = cslot + 1 == FW_AHEAD ? 0 : cslot + 1;
+    cslot = (cslot + 1) % FW_AHEAD;
   };
   if (mine > 0) {
     open_job();
@@ -318,21 +309,22 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
 #pragma unroll
         for (int i = 0; i < SUBS; ++i) sc[r][i] = sm.scale[warp][slot][r][g * SUBS + i];
       }
-      slot = slot + 1 == FW_AHEAD ? 0 : slot + 1;
+      slot = (slot + 1) % FW_AHEAD;
 #pragma unroll
       for (int i = 0; i < SUBS; ++i) {
         float start[4];  // - (B + 8) sum x, by token column
-        const uint32_t ones[4] = {ONES, ONES, ONES, ONES};
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t offset[4] = {OFFSET, OFFSET, OFFSET, OFFSET};
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           const uint4 xv = x[(i * PER + k) >> 1][(i * PER + k) & 1];
-          mma_16816<T>(start, ones, xv.x, xv.y, k == 0);
-          mma_16816<T>(start, ones, xv.z, xv.w, false);
+          if (k == 0) mma_16816<T>(start, offset, xv.x, xv.y, zero);
+          else mma_16816<T>(start, offset, xv.x, xv.y, start);
+          mma_16816<T>(start, offset, xv.z, xv.w, start);
         }
-        const float s0 = START * start[0], s1 = START * start[1];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float d[4] = {s0, s1, s0, s1};
+          float d[4];
 #pragma unroll
           for (int k = 0; k < PER; ++k) {
             const int bl = (i * PER + k) >> 1, h = (i * PER + k) & 1;
@@ -342,7 +334,8 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
             for (int m = 0; m < 2; ++m) {
               const uint32_t fr[4] = {rf::int4_raw<T>(lo, 2 * m), rf::int4_raw<T>(hi, 2 * m),
                                       rf::int4_raw<T>(lo, 2 * m + 1), rf::int4_raw<T>(hi, 2 * m + 1)};
-              mma_16816<T>(d, fr, m ? xv.z : xv.x, m ? xv.w : xv.y, false);
+              if (k + m == 0) mma_16816<T>(d, fr, xv.x, xv.y, start);
+              else mma_16816<T>(d, fr, m ? xv.z : xv.x, m ? xv.w : xv.y, d);
             }
           }
           const float2 f = scale_pair<T>(sc[r][i]);

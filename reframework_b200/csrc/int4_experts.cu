@@ -37,6 +37,7 @@ constexpr int FW_THREADS = FW_WARPS * 32;
 constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
 constexpr int FW_STEP = rf::I4_STEP;
 constexpr int FW_AHEAD = 4;     // a power of two: ring slots of a warp: steps of codes on their way, and the one in use
+constexpr int FW_MANY_JOBS = 2368;  // 32-row units from which two warps share a unit's k instead of eight
 constexpr int KMAX = 16;
 
 struct FewArgs {
@@ -45,7 +46,7 @@ struct FewArgs {
   const void *scales;
   void *out;             // h [pairs, N] in T (gated) or y [pairs, N] fp32
   const int32_t *ids;    // [pairs]
-  int pairs, topk, E, N, Kd, act, units;
+  int pairs, topk, E, N, Kd, act, units;  // units: 32-row units times the row groups of a job, rounded up
   rf::Int4Shape sh;
 };
 
@@ -54,12 +55,12 @@ template <typename T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                           const float (&c)[4]) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
@@ -87,8 +88,8 @@ struct FewShared {
   int active, part[FW_WARPS];
 };
 
-// A job is 32 weight rows of one expert against 8 of its tokens; a launch's jobs
-// in the order expert, unit (of 32 rows), pass (of 8 tokens).
+// A job is 32 weight rows for each of the block's row groups, of one expert,
+// against 8 of its tokens; a launch's jobs in the order expert, unit, pass.
 struct FewJob {
   int y, unit, pass;
 };
@@ -161,7 +162,8 @@ __device__ __forceinline__ void copy_bytes(uint32_t dst, const void *src) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// SUBS: scale groups in a step's 128 k (1, 2 or 4).
+// SUBS: scale groups in a step's 128 k (1, 2 or 4).  KS: warps that share a
+// row group's k; the block's 8 / KS row groups are 32 weight rows each.
 //
 // The codes go to the tensor cores as code + B (B = 128 in bf16, 1024 in fp16:
 // a shift and one three-input logic operation per pair), and a group's sums
@@ -174,7 +176,7 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile
 // Each warp copies its codes into a ring of its own, FW_AHEAD - 1 steps before
 // their use and across the ends of jobs: a job is only a few steps long per
 // warp (4 at K = 4096), and the memory would idle at each end.
-template <typename T, bool GATED, int SUBS>
+template <typename T, bool GATED, int SUBS, int KS>
 __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
   extern __shared__ __align__(16) uint8_t few_smem[];
   FewShared &sm = *reinterpret_cast<FewShared *>(few_smem);
@@ -198,7 +200,9 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
   const int j0 = (int)(jobs * blockIdx.x / gridDim.x), j1 = (int)(jobs * (blockIdx.x + 1) / gridDim.x);
   if (j0 >= j1) return;
   const int steps = (int)p.sh.k_blocks / 2;
-  const int st0 = steps * warp / FW_WARPS, mine = steps * (warp + 1) / FW_WARPS - st0;  // this warp's steps of a job
+  constexpr int RG = FW_WARPS / KS;
+  const int rg = warp / KS, ks = warp % KS;
+  const int st0 = steps * ks / KS, mine = steps * (ks + 1) / KS - st0;  // this warp's steps of a job
 
   auto passes_of = [&](int y) { return sm.prefix[y + 1] - sm.prefix[y]; };
   auto job_at = [&](int j) {
@@ -228,8 +232,10 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
     if (cj >= j1) return;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      int64_t rb = GATED ? cb.unit + r * p.sh.half_blocks : 2 * (int64_t)cb.unit + r;
-      rb = (int64_t)sm.expert[cb.y] * p.sh.row_blocks() + min(rb, p.sh.row_blocks() - 1);
+      // rows past the weight's own read its last block: never stored
+      const int64_t u = cb.unit * RG + rg;
+      int64_t rb = GATED ? min(u, p.sh.half_blocks - 1) + r * p.sh.half_blocks : min(2 * u + r, p.sh.half_blocks - 1);
+      rb += (int64_t)sm.expert[cb.y] * p.sh.row_blocks();
       wp[r] = reinterpret_cast<const uint4 *>(p.w + (rb * p.sh.k_blocks + 2 * st0) * rf::I4_BLOCK) + lane;
       sp[r] = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(p.scales) +
                                                  (rb * p.sh.groups + st0 * SUBS) * rf::I4_ROWS) + g * SUBS;
@@ -353,25 +359,27 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
 #pragma unroll
       for (int i = 0; i < 4; ++i) sm.red[warp][(r * 4 + i) * 32 + lane] = acc[r][i];
     __syncthreads();
-    constexpr int PER = GATED ? 16 : 32;  // features of a unit
-    const int f = threadIdx.x % PER, col = threadIdx.x / PER;  // feature, token of the job
-    const int r16 = f & 15;
-    const int at = ((col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + (col >> 1);
-    const int64_t feat = (int64_t)b.unit * PER + f;
-    if (col < 8 && c0 + col < cnt && feat < p.N) {
+    constexpr int PER = GATED ? 16 : 32;  // features of a row group
+#pragma unroll
+    for (int i = threadIdx.x; i < RG * PER * 8; i += FW_THREADS) {
+      const int f = i % (RG * PER), col = i / (RG * PER);  // feature, token of the job
+      const int r16 = f & 15, w0 = f / PER * KS;
+      const int at = ((col & 1) + 2 * (r16 >> 3)) * 32 + (r16 & 7) * 4 + (col >> 1);
+      const int64_t feat = (int64_t)b.unit * (RG * PER) + f;
+      if (c0 + col >= cnt || feat >= p.N) continue;
       const int64_t row = sm.list[c0 + col];
       if constexpr (GATED) {
         float gt = 0.f, up = 0.f;
 #pragma unroll
-        for (int w = 0; w < FW_WARPS; ++w) {
-          gt += sm.red[w][at];
-          up += sm.red[w][at + 4 * 32];
+        for (int w = 0; w < KS; ++w) {
+          gt += sm.red[w0 + w][at];
+          up += sm.red[w0 + w][at + 4 * 32];
         }
         reinterpret_cast<T *>(p.out)[row * p.N + feat] = rf::Cvt<T>::from_f(rf::act_gate(p.act, gt) * up);
       } else {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < FW_WARPS; ++w) v += sm.red[w][at + (f >> 4) * 4 * 32];
+        for (int w = 0; w < KS; ++w) v += sm.red[w0 + w][at + (f >> 4 & 1) * 4 * 32];
         reinterpret_cast<float *>(p.out)[row * p.N + feat] = v;
       }
     }
@@ -402,9 +410,9 @@ int launch_chained(const char *what, void (*kern)(Params...), dim3 grid, int thr
   return RF_OK;
 }
 
-template <typename T, bool GATED, int SUBS>
-int launch_few_s(const FewArgs &p, cudaStream_t st) {
-  auto kern = int4_few_kernel<T, GATED, SUBS>;
+template <typename T, bool GATED, int SUBS, int KS>
+int launch_few_k(FewArgs p, cudaStream_t st) {
+  auto kern = int4_few_kernel<T, GATED, SUBS, KS>;
   const char *what = GATED ? "4-bit gated products (few rows)" : "4-bit down products (few rows)";
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
@@ -417,10 +425,18 @@ int launch_few_s(const FewArgs &p, cudaStream_t st) {
     cudaGetLastError();
     return rf::fail(RF_ERR_CUDA, std::string(what) + ": the kernel does not fit this device");
   }
+  p.units = (p.units + FW_WARPS / KS - 1) / (FW_WARPS / KS);
   // as many blocks as run at once share the jobs (at most units * pairs) evenly
   const int64_t most = (int64_t)p.units * p.pairs;
   const int64_t blocks = std::min<int64_t>(most, (int64_t)rf::num_sms() * resident);
   return launch_chained(what, kern, dim3((unsigned)blocks), FW_THREADS, sizeof(FewShared), !GATED, st, p);
+}
+
+template <typename T, bool GATED, int SUBS>
+int launch_few_s(const FewArgs &p, cudaStream_t st) {
+  const int64_t jobs = (int64_t)p.units * std::min(p.E, p.pairs);
+  if (jobs >= FW_MANY_JOBS) return launch_few_k<T, GATED, SUBS, 2>(p, st);
+  return launch_few_k<T, GATED, SUBS, 8>(p, st);
 }
 
 template <typename T, bool GATED>

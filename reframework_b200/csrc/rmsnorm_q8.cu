@@ -11,11 +11,9 @@
 // HBM-bound: each input element is read once and kept in registers across the
 // two reductions (sum of squares, then max|z|), each output written once.  The
 // sums and z are fp32; the roundings are those of the outputs' types.  A row
-// belongs to one warp (up to 128 16-byte vectors) or to one block; the threads
-// keep their columns' weights in registers over all rows that they take.
+// belongs to TPR threads (a warp, or a small block) with up to four 16-byte
+// vectors each: few threads per barrier, many independent rows per SM.
 #include <cuda_fp8.h>
-
-#include <algorithm>
 
 #include "common.cuh"
 
@@ -48,7 +46,6 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   if constexpr (TPR > 32) {
-    __syncthreads();
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.f;
@@ -58,25 +55,34 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
   return v;
 }
 template <int TPR>
-__device__ __forceinline__ float row_max(float v, float *red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
+  v = __reduce_max_sync(FULL, v);
   if constexpr (TPR > 32) {
-    __syncthreads();
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < TPR / 32; ++w) v = fmaxf(v, red[w]);
+    for (int w = 1; w < TPR / 32; ++w) v = max(v, red[w]);
   }
   return v;
 }
 
-// max|z| of a group -> its scale; a non-finite value was turned into +inf.
-__device__ __forceinline__ float scale_of(float amax) {
-  if (amax == 0.f) return 1.f;
-  if (!(amax < INFINITY)) return NAN;
-  return fmaxf(amax / E4M3_MAX, MIN_SCALE);
+// Magnitudes are compared as the integers of their bits: the same order, and a
+// NaN (above the infinity's bits) is not lost as in a float maximum.
+constexpr uint32_t INF_BITS = 0x7f800000u;
+__device__ __forceinline__ uint32_t mag_bits(float z) { return __float_as_uint(z) & 0x7fffffffu; }
+
+// max|z| of a group -> its scale, and 1 / scale (0 for a group that is not finite).
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  if (top == 0u) return 1.f;
+  if (top >= INF_BITS) return NAN;
+  return fmaxf(__uint_as_float(top) / E4M3_MAX, MIN_SCALE);
+}
+__device__ __forceinline__ float inverse_of(uint32_t top) {
+  const float amax = __uint_as_float(top);
+  if (amax > 0x1p-100f && amax < 0x1p100f) return __fdividef(E4M3_MAX, amax);  // within 2 ulp
+  if (top >= INF_BITS) return 0.f;
+  return top == 0u ? 1.f : 1.0f / scale_of(top);
 }
 
 template <typename T, int V>
@@ -89,76 +95,97 @@ __device__ __forceinline__ void store_vec(T *p, const float *f) {
   }
 }
 
+template <int V>
+__device__ __forceinline__ void load_f32(const float *p, int at, float (&f)[V]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + at + i));
+      f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = __ldg(p + at + i);
+  }
+}
+
 __device__ __forceinline__ uint32_t e4m3x4(const float *z, float inv) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(z[0] * inv, z[1] * inv), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z[2] * inv, z[3] * inv), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
 
-// TPR threads per row, VPT 16-byte vectors per thread; a warp-row block holds
-// ROWS rows.
+// TPR threads per row, VPT 16-byte vectors per thread; a block holds one row,
+// or four where a row is a warp's.
 template <typename T, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) add_rmsnorm_q8_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rmsnorm_q8_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(T);
-  constexpr int ROWS = TPR == 32 ? 8 : 1;
-  __shared__ float red[TPR / 32];
+  __shared__ float sum_red[TPR / 32];
+  __shared__ uint32_t max_red[TPR / 32];
   const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const int nvec = a.H / V;
-  float w[VPT][V];
-#pragma unroll
-  for (int u = 0; u < VPT; ++u) {
-    const int v = tid + u * TPR;
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[u][i] = v < nvec ? a.w[v * V + i] : 0.f;
-  }
   const T *x = reinterpret_cast<const T *>(a.x);
   const T *res = reinterpret_cast<const T *>(a.residual);
-  const int64_t step = (int64_t)gridDim.x * ROWS;
-  for (int64_t t = (int64_t)blockIdx.x * ROWS + (TPR == 32 ? threadIdx.x >> 5 : 0); t < a.T; t += step) {
+  const int64_t t = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (t >= a.T) return;
+  {
     float z[VPT][V];
+    uint4 xv[VPT], rv[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int v = tid + u * TPR;
+      const int64_t at = t * a.H + (int64_t)v * V;
+      xv[u] = v < nvec ? __ldg(reinterpret_cast<const uint4 *>(x + at)) : make_uint4(0u, 0u, 0u, 0u);
+      if (res) rv[u] = v < nvec ? __ldg(reinterpret_cast<const uint4 *>(res + at)) : make_uint4(0u, 0u, 0u, 0u);
+    }
     float ss = 0.f;
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
       const int v = tid + u * TPR;
-      const bool ok = v < nvec;
-      const int64_t at = t * a.H + (int64_t)v * V;
-      rf::unpack16<T>(ok ? __ldg(reinterpret_cast<const uint4 *>(x + at)) : make_uint4(0u, 0u, 0u, 0u), z[u]);
+      rf::unpack16<T>(xv[u], z[u]);
       if (res) {
         float f[V];
-        rf::unpack16<T>(ok ? __ldg(reinterpret_cast<const uint4 *>(res + at)) : make_uint4(0u, 0u, 0u, 0u), f);
+        rf::unpack16<T>(rv[u], f);
 #pragma unroll
         for (int i = 0; i < V; ++i) z[u][i] = rf::round_to<T>(__fadd_rn(z[u][i], f[i]));
       }
-      if (a.residual_out && ok) store_vec<T, V>(reinterpret_cast<T *>(a.residual_out) + at, z[u]);
+      if (a.residual_out && v < nvec)
+        store_vec<T, V>(reinterpret_cast<T *>(a.residual_out) + t * a.H + (int64_t)v * V, z[u]);
 #pragma unroll
       for (int i = 0; i < V; ++i) ss = fmaf(z[u][i], z[u][i], ss);
     }
-    const float inv = 1.0f / sqrtf(row_sum<TPR>(ss, red) / (float)a.H + a.eps);
-    float amax = 0.f;  // of this thread's columns (the whole row is one group)
-    float vmax[VPT];   // of one vector
+    const float inv = 1.0f / sqrtf(row_sum<TPR>(ss, sum_red) / (float)a.H + a.eps);
+    uint32_t top = 0u;  // of this thread's columns (the whole row is one group)
+    uint32_t vmax[VPT]; // of one vector
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
       const int v = tid + u * TPR;
-      vmax[u] = 0.f;
+      vmax[u] = 0u;
+      if (v < nvec) {
+        float w[V], bias[V];
+        load_f32<V>(a.w, v * V, w);
+        if (a.b) load_f32<V>(a.b, v * V, bias);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        z[u][i] = z[u][i] * inv * w[u][i];
-        if (a.b && v < nvec) z[u][i] += a.b[v * V + i];
-        // a NaN counts as an infinity (fmaxf would drop it); lanes past the row hold 0 * inv
-        const float m = v < nvec ? fabsf(z[u][i]) : 0.f;
-        vmax[u] = fmaxf(vmax[u], m == m ? m : INFINITY);
+        for (int i = 0; i < V; ++i) {
+          z[u][i] = z[u][i] * inv * w[i];
+          if (a.b) z[u][i] += bias[i];
+          vmax[u] = max(vmax[u], mag_bits(z[u][i]));
+        }
       }
-      amax = fmaxf(amax, vmax[u]);
+      top = max(top, vmax[u]);
     }
+    float is[VPT];
     if (a.lanes == 0) {
-      amax = row_max<TPR>(amax, red);
+      top = row_max<TPR>(top, max_red);
+      is[0] = inverse_of(top);
 #pragma unroll
-      for (int u = 0; u < VPT; ++u) vmax[u] = amax;
-      if (tid == 0 && a.q) a.scales[t] = scale_of(amax);
+      for (int u = 1; u < VPT; ++u) is[u] = is[0];
+      if (tid == 0 && a.q) a.scales[t] = scale_of(top);
     } else {
 #pragma unroll
       for (int u = 0; u < VPT; ++u) {
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) vmax[u] = fmaxf(vmax[u], __shfl_xor_sync(FULL, vmax[u], o));
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) vmax[u] = max(vmax[u], __shfl_xor_sync(FULL, vmax[u], o));
+        is[u] = inverse_of(vmax[u]);
         const int v = tid + u * TPR;
         if (v < nvec && v % a.lanes == 0 && a.q) a.scales[t * a.n_groups + v / a.lanes] = scale_of(vmax[u]);
       }
@@ -170,12 +197,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) add_rmsnorm_q8_kernel(c
       const int64_t at = t * a.H + (int64_t)v * V;
       if (a.normed) store_vec<T, V>(reinterpret_cast<T *>(a.normed) + at, z[u]);
       if (!a.q) continue;
-      const float scale = scale_of(vmax[u]);
-      const bool fine = scale == scale;
-      const float is = 1.0f / scale;
       uint32_t q[V / 4];
 #pragma unroll
-      for (int i = 0; i < V / 4; ++i) q[i] = fine ? e4m3x4(z[u] + 4 * i, is) : 0u;
+      for (int i = 0; i < V / 4; ++i) q[i] = is[u] != 0.f ? e4m3x4(z[u] + 4 * i, is[u]) : 0u;
       if constexpr (V == 8) *reinterpret_cast<uint2 *>(a.q + at) = make_uint2(q[0], q[1]);
       else *reinterpret_cast<uint32_t *>(a.q + at) = q[0];
     }
@@ -184,10 +208,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) add_rmsnorm_q8_kernel(c
 
 template <typename T, int TPR, int VPT>
 int launch_v(const NormArgs &a, cudaStream_t st) {
-  constexpr int ROWS = TPR == 32 ? 8 : 1;
-  constexpr int THREADS = TPR == 32 ? 256 : TPR;
-  const int64_t blocks = std::min<int64_t>((a.T + ROWS - 1) / ROWS, (int64_t)rf::num_sms() * (2048 / THREADS));
-  add_rmsnorm_q8_kernel<T, TPR, VPT><<<(int)blocks, THREADS, 0, st>>>(a);
+  constexpr int ROWS = TPR == 32 ? 4 : 1;
+  const int64_t blocks = (a.T + ROWS - 1) / ROWS;
+  add_rmsnorm_q8_kernel<T, TPR, VPT><<<(unsigned)blocks, TPR == 32 ? 128 : TPR, 0, st>>>(a);
   return rf::check_launch("rf_moe_add_rmsnorm_q8");
 }
 
@@ -196,13 +219,12 @@ int launch_t(const NormArgs &a, cudaStream_t st) {
   const int nvec = a.H / (16 / (int)sizeof(T));
   if (nvec <= 32) return launch_v<T, 32, 1>(a, st);
   if (nvec <= 64) return launch_v<T, 32, 2>(a, st);
-  if (nvec <= 128) return launch_v<T, 128, 1>(a, st);
-  if (nvec <= 256) return launch_v<T, 256, 1>(a, st);
-  if (nvec <= 512) return launch_v<T, 256, 2>(a, st);
-  if (nvec <= 1024) return launch_v<T, 512, 2>(a, st);
-  if (nvec <= 2048) return launch_v<T, 1024, 2>(a, st);
-  if (nvec <= 4096) return launch_v<T, 1024, 4>(a, st);
-  return rf::fail(RF_ERR_UNSUPPORTED, "rf_moe_add_rmsnorm_q8: a row holds at most 65536 bytes");
+  if (nvec <= 128) return launch_v<T, 32, 4>(a, st);
+  if (nvec <= 256) return launch_v<T, 64, 4>(a, st);
+  if (nvec <= 512) return launch_v<T, 128, 4>(a, st);
+  if (nvec <= 1024) return launch_v<T, 256, 4>(a, st);
+  if (nvec <= 2048) return launch_v<T, 512, 4>(a, st);
+  return launch_v<T, 1024, 4>(a, st);  // up to 65536 bytes
 }
 
 }  // namespace
@@ -212,7 +234,7 @@ extern "C" int rf_moe_add_rmsnorm_q8(const void *x, const void *residual, int64_
                                      int64_t group_size, void *residual_out, void *normed_out, void *q,
                                      float *scales, rf_stream_t stream) {
   RF_CHECK_ARG(rf::valid_dtype(dtype), "rf_moe_add_rmsnorm_q8: unknown dtype");
-  RF_CHECK_ARG(T >= 0 && H > 0 && H < ((int64_t)1 << 30), "rf_moe_add_rmsnorm_q8: bad sizes");
+  RF_CHECK_ARG(T >= 0 && T <= 0x7fffffff && H > 0 && H < ((int64_t)1 << 30), "rf_moe_add_rmsnorm_q8: bad sizes");
   const int64_t esz = (int64_t)rf::dtype_size(dtype);
   RF_CHECK_ARG((H * esz) % 16 == 0, "rf_moe_add_rmsnorm_q8: H * element size must be a multiple of 16 bytes");
   RF_CHECK_ARG(eps >= 0.f, "rf_moe_add_rmsnorm_q8: eps must be >= 0");

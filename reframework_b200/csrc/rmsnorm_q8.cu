@@ -41,28 +41,29 @@ struct NormArgs {
   float eps;
 };
 
-template <int TPR>
+// Over the threads of a row: a warp, or the block's warps in warp order.
+template <int WARPS>
 __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-  if constexpr (TPR > 32) {
+  if constexpr (WARPS > 1) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) v += red[w];
+    for (int w = 0; w < WARPS; ++w) v += red[w];
   }
   return v;
 }
-template <int TPR>
+template <int WARPS>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
   v = __reduce_max_sync(FULL, v);
-  if constexpr (TPR > 32) {
+  if constexpr (WARPS > 1) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < TPR / 32; ++w) v = max(v, red[w]);
+    for (int w = 1; w < WARPS; ++w) v = max(v, red[w]);
   }
   return v;
 }
@@ -115,18 +116,19 @@ __device__ __forceinline__ uint32_t e4m3x4(const float *z, float inv) {
   return lo | (hi << 16);
 }
 
-// TPR threads per row, VPT 16-byte vectors per thread; a block holds one row,
-// or four where a row is a warp's.
-template <typename T, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rmsnorm_q8_kernel(const NormArgs a) {
+// WARPS warps per row, up to VPT 16-byte vectors per thread; a block holds one
+// row, or four where a row is a warp's.
+template <typename T, int WARPS, int VPT>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) add_rmsnorm_q8_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(T);
-  __shared__ float sum_red[TPR / 32];
-  __shared__ uint32_t max_red[TPR / 32];
-  const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  constexpr int TPR = WARPS * 32;  // threads of a row
+  __shared__ float sum_red[WARPS];
+  __shared__ uint32_t max_red[WARPS];
+  const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
   const int nvec = a.H / V;
   const T *x = reinterpret_cast<const T *>(a.x);
   const T *res = reinterpret_cast<const T *>(a.residual);
-  const int64_t t = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  const int64_t t = WARPS == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
   if (t >= a.T) return;
   {
     float z[VPT][V];
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rmsnorm_q8_kernel(c
 #pragma unroll
       for (int i = 0; i < V; ++i) ss = fmaf(z[u][i], z[u][i], ss);
     }
-    const float inv = 1.0f / sqrtf(row_sum<TPR>(ss, sum_red) / (float)a.H + a.eps);
+    const float inv = 1.0f / sqrtf(row_sum<WARPS>(ss, sum_red) / (float)a.H + a.eps);
     uint32_t top = 0u;  // of this thread's columns (the whole row is one group)
     uint32_t vmax[VPT]; // of one vector
 #pragma unroll
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rmsnorm_q8_kernel(c
     }
     float is[VPT];
     if (a.lanes == 0) {
-      top = row_max<TPR>(top, max_red);
+      top = row_max<WARPS>(top, max_red);
       is[0] = inverse_of(top);
 #pragma unroll
       for (int u = 1; u < VPT; ++u) is[u] = is[0];
@@ -206,25 +208,40 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rmsnorm_q8_kernel(c
   }
 }
 
-template <typename T, int TPR, int VPT>
+template <typename T, int WARPS, int VPT>
 int launch_v(const NormArgs &a, cudaStream_t st) {
-  constexpr int ROWS = TPR == 32 ? 4 : 1;
-  const int64_t blocks = (a.T + ROWS - 1) / ROWS;
-  add_rmsnorm_q8_kernel<T, TPR, VPT><<<(unsigned)blocks, TPR == 32 ? 128 : TPR, 0, st>>>(a);
+  const int64_t blocks = WARPS == 1 ? (a.T + 3) / 4 : a.T;
+  add_rmsnorm_q8_kernel<T, WARPS, VPT><<<(unsigned)blocks, WARPS == 1 ? 128 : WARPS * 32, 0, st>>>(a);
   return rf::check_launch("rf_moe_add_rmsnorm_q8");
 }
 
+// Few rows leave SMs idle, so a row gets twice the threads (64 rows of 4096:
+// 3.5 us against 4.2); with many, four vectors a thread keep more bytes in
+// flight for each barrier (2047 rows of 6144: 15.8 us against 19.1).
 template <typename T>
 int launch_t(const NormArgs &a, cudaStream_t st) {
   const int nvec = a.H / (16 / (int)sizeof(T));
-  if (nvec <= 32) return launch_v<T, 32, 1>(a, st);
-  if (nvec <= 64) return launch_v<T, 32, 2>(a, st);
-  if (nvec <= 128) return launch_v<T, 32, 4>(a, st);
-  if (nvec <= 256) return launch_v<T, 64, 4>(a, st);
-  if (nvec <= 512) return launch_v<T, 128, 4>(a, st);
-  if (nvec <= 1024) return launch_v<T, 256, 4>(a, st);
-  if (nvec <= 2048) return launch_v<T, 512, 4>(a, st);
-  return launch_v<T, 1024, 4>(a, st);  // up to 65536 bytes
+  if (nvec <= 32) return launch_v<T, 1, 1>(a, st);
+  if (nvec <= 64) return launch_v<T, 1, 2>(a, st);
+  if (a.T <= 2 * rf::num_sms() && nvec <= 1024) {
+    if (nvec <= 128) return launch_v<T, 2, 2>(a, st);
+    if (nvec <= 256) return launch_v<T, 4, 2>(a, st);
+    if (nvec <= 512) return launch_v<T, 8, 2>(a, st);
+    return launch_v<T, 16, 2>(a, st);
+  }
+  switch ((nvec + 127) / 128) {
+    case 1: return launch_v<T, 1, 4>(a, st);
+    case 2: return launch_v<T, 2, 4>(a, st);
+    case 3: return launch_v<T, 3, 4>(a, st);
+    case 4: return launch_v<T, 4, 4>(a, st);
+    case 5: return launch_v<T, 5, 4>(a, st);
+    case 6: return launch_v<T, 6, 4>(a, st);
+    case 7: return launch_v<T, 7, 4>(a, st);
+    case 8: return launch_v<T, 8, 4>(a, st);
+    default: break;
+  }
+  if (nvec <= 2048) return launch_v<T, 16, 4>(a, st);
+  return launch_v<T, 32, 4>(a, st);  // up to 65536 bytes
 }
 
 }  // namespace

@@ -11,20 +11,21 @@
 //   ids = the K largest c, in that order (ties: the lower id; a NaN c counts as
 //   -inf); w = s[ids], divided by max(sum w, 1e-20) when renormalising, * scale
 //
-// The order is that of the exact scores, not of their fp32 roundings:
-//   * without a bias c is monotone in l, so experts (and groups by their
-//     maximum) are compared by their logits, which are exact;
-//   * otherwise c is computed in fp32 with a bound on its error, and a token
-//     whose decision hangs on a gap within that bound is decided again in fp64
-//     (route_exact: one token in some thousands, at its warp's expense alone).
-// One warp per token: lane i holds the nv consecutive experts from i * nv, in
-// registers, nv being a divisor of the group size wherever one fits, so that a
-// group is a run of whole lanes: its score is a segmented shuffle reduction,
-// and a choice is one redux.sync over order-preserving integer keys, the
-// lowest lane with the largest key holding the lowest id.  (Sizes without such
-// an nv, e.g. groups of 37, take the fp64 form for every token.)
-#include <algorithm>
-
+// The order is that of the exact scores, not of their fp32 roundings: experts
+// are picked by fp32 values with a bound on their error, and where a decision
+// hangs on a gap within that bound the candidates are put in order by their
+// fp64 scores (without a bias c is monotone in l, so logits are compared then).
+// The weights are computed from the chosen logits alone, to full fp32 accuracy.
+//
+// One warp per token: lane i holds the nv consecutive experts from i * nv as
+// order-preserving integer keys, sorted, nv being a divisor of the group size
+// wherever one fits, so that a group is a run of whole lanes and its score a
+// segmented shuffle reduction over the lanes' first keys.  A pick is one
+// redux.sync over the lanes' first keys and a shift in the lane that had it.
+// The place within a lane is kept in a key's low bits (part of the error
+// bound).  Sizes without such an nv, e.g. groups of 37, take an fp64 form.
+// Bound by issuing instructions: about 600 a token for 256 experts and K = 8,
+// of which 8 sigmoids a lane, a sort of 8 and 9 picks.
 #include "router.cuh"
 
 RF_DEVICE_ERROR_WORD();
@@ -38,8 +39,9 @@ constexpr uint32_t KEY_NEG_INF = 0x007fffffu;  // order_key(-inf)
 // Keys below it: 0 for a taken expert or a place past E, and KEY_MASKED for a
 // NaN or a dropped group where logits are compared (there -inf stands for a
 // score of 0, which comes before a masked one).  Where scores are compared
-// NaN and dropped groups are -inf itself, like a closed expert.
-constexpr uint32_t KEY_MASKED = 1u;
+// NaN and dropped groups are -inf itself, like a closed expert.  (64: above the
+// place bits.)
+constexpr uint32_t KEY_MASKED = 64u;
 
 struct GroupedArgs {
   const void *x;         // logits [T, E] when partial is NULL
@@ -172,7 +174,7 @@ __device__ __noinline__ void route_exact(const GroupedArgs &a, int64_t t, double
   *my_s = lane < a.K ? (float)score_of((double)logit_of<TX>(a, t, id)) : 0.f;
 }
 
-// nv consecutive logits from element e of row t (e a multiple of nv).
+// nv consecutive logits from element e0 of row t.
 template <int NV, typename TX>
 __device__ __forceinline__ void load_logits(const GroupedArgs &a, int64_t t, int e0, int nv, float (&l)[NV]) {
   constexpr int V = 16 / sizeof(TX);
@@ -203,196 +205,240 @@ __device__ __forceinline__ void load_logits(const GroupedArgs &a, int64_t t, int
     if (j < nv && e0 + j < a.E) l[j] = logit_of<TX>(a, t, e0 + j);
 }
 
+// Descending, NV a power of two (bitonic: every comparison a min and a max).
+template <int NV>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[NV]) {
+#pragma unroll
+  for (int size = 2; size <= NV; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = i ^ d;
+        if (j > i) {
+          const uint32_t hi = max(k[i], k[j]), lo = min(k[i], k[j]);
+          const bool down = (i & size) == 0;
+          k[i] = down ? hi : lo;
+          k[j] = down ? lo : hi;
+        }
+      }
+}
+
+// A score to within 7 * 2^-24 (sigmoid): __expf is off by (2 + 1.173 |l|) ulp,
+// of which the score sees s (1 - s), at most 0.77 ulp of 1 in all; the quotient
+// adds 2 and the sum half an ulp.
+__device__ __forceinline__ float fast_sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
+
 template <int NV, typename TX>
 __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const GroupedArgs a) {
   extern __shared__ double s_exact[];  // [GR_WARPS][E], for route_exact
+  constexpr uint32_t PLACE = NV - 1;   // the low bits of a key: NV - 1 - place in the lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nv = a.nv;
   const int e0 = lane * nv;
   const bool by_score = a.select_bias != nullptr;  // else experts are compared by their logits
-  const bool group_by_score = by_score || a.top2;
-  const uint32_t low = by_score ? KEY_NEG_INF : KEY_MASKED;
-  for (int64_t t = (int64_t)blockIdx.x * GR_WARPS + warp; t < a.T; t += (int64_t)gridDim.x * GR_WARPS) {
-    if (a.has_shared && lane == 0) {
-      const float z = rf::sum_slices(a.partial + t * a.ld + a.E, a.T * a.ld, a.slices);
-      a.shared_scale[t] = 1.0f / (1.0f + expf(-z));
+  const uint32_t low = (by_score ? KEY_NEG_INF : KEY_MASKED) & ~PLACE;
+  const int64_t t = (int64_t)blockIdx.x * GR_WARPS + warp;
+  if (t >= a.T) return;
+  if (a.has_shared && lane == 0) {
+    const float z = rf::sum_slices(a.partial + t * a.ld + a.E, a.T * a.ld, a.slices);
+    a.shared_scale[t] = 1.0f / (1.0f + expf(-z));
+  }
+  if (a.logits_out)
+    for (int e = lane; e < a.E; e += 32) a.logits_out[t * a.E + e] = logit_of<TX>(a, t, e);
+  int my_id = 0;
+  float my_s = 0.f;
+  bool exact = nv == 0;  // every decision of this token in fp64
+  float m = 0.f, sum = 1.f;  // softmax: the largest logit, the sum
+  if (!exact) {
+    float l[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) l[j] = -INFINITY;
+    load_logits<NV, TX>(a, t, e0, nv, l);
+    bool row_nan = false;
+    if (!a.sigmoid) {
+      m = l[0];
+#pragma unroll
+      for (int j = 1; j < NV; ++j) m = fmaxf(m, l[j]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+      sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) sum += j < nv && e0 + j < a.E ? __expf(l[j] - m) : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+      row_nan = !(sum == sum);
     }
-    if (a.logits_out)
-      for (int e = lane; e < a.E; e += 32) a.logits_out[t * a.E + e] = logit_of<TX>(a, t, e);
-    int my_id = 0;
-    float my_s = 0.f;
-    bool exact = nv == 0;
-    if (!exact) {
-      // ---- scores
-      float l[NV], s[NV];
-      uint32_t key[NV];
+    // Errors, absolute: of a score (softmax: __expf within 2 + 1.173 |l - m| ulp
+    // and its argument's rounding, worth 3 ulp of the largest score; the sum's,
+    // with |l - m| at most 8 on average, and its NV + 5 additions; a product),
+    // of c's own rounding, and of the place bits in a key.
+    const float inv = 1.0f / sum;
+    const float eps = a.sigmoid ? 7.f * 0x1p-24f : (NV + 48) * 0x1p-24f * inv;
+    constexpr float KEY_EPS = (NV > 1 ? 2 * NV : 1) * 0x1p-24f;  // relative, with a rounding
+    // ---- keys
+    uint32_t key[NV];
+    float cabs = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) l[j] = -INFINITY;
-      load_logits<NV, TX>(a, t, e0, nv, l);
-      float eps, smax;  // relative error of a score (see below), an upper bound of the scores
-      bool row_nan = false;
-      if (a.sigmoid) {
-        smax = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          s[j] = 1.0f / (1.0f + expf(-l[j]));
-          smax = fmaxf(smax, s[j]);
-        }
-        // expf within 2 ulp, one addition, one division
-        eps = 6.0f * 0x1p-24f;
-      } else {
-        float m = l[0];
-#pragma unroll
-        for (int j = 1; j < NV; ++j) m = fmaxf(m, l[j]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          s[j] = j < nv && e0 + j < a.E ? expf(l[j] - m) : 0.f;
-          sum += s[j];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
-        row_nan = !(sum == sum);
-        smax = 1.0f / sum;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) s[j] = s[j] / sum;
-        // expf within 2 ulp (its argument's own rounding is worth less than
-        // one more: x e^-x < 0.37), NV + 5 additions, one division
-        eps = (NV + 5 + 8) * 0x1p-24f;
-      }
-      // ---- what experts are compared by
-      float cabs = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int e = e0 + j;
-        float c = l[j];
-        if (by_score && j < nv && e < a.E) c = s[j] + a.select_bias[e];
-        if (fabsf(c) < INFINITY) cabs = fmaxf(cabs, fabsf(c));
-        key[j] = j < nv && e < a.E ? (row_nan ? low : order_key(c, low)) : 0u;
-      }
-      // Two fp32 scores closer than tol may be in the other order exactly:
-      // each is off by at most eps * smax + 2^-24 * |c|.
-      float tol = -1.f, gtol = -1.f;
-      if (group_by_score) {
-        smax = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(fmaxf(smax, 0.f))));
-        cabs = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(by_score ? cabs : smax)));
-        const float one = eps * smax + 0x1p-24f * cabs;
-        if (by_score) tol = 2.f * one;
-        gtol = a.top2 ? 4.f * one + 0x1p-22f * cabs : 2.f * one;
-      }
-      // ---- groups: runs of `lanes` lanes
-      if (a.G > 1) {
-        const int lanes = a.per / nv;
-        uint32_t k1 = 0u;       // by maximum, as keys
-        float c1 = -INFINITY, c2 = -INFINITY;  // by the two largest
-        if (!a.top2) {
-#pragma unroll
-          for (int j = 0; j < NV; ++j) k1 = max(k1, key[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const float c = key[j] > low ? (by_score ? key_value(key[j]) : s[j]) : -INFINITY;
-            c2 = fmaxf(c2, fminf(c1, c));
-            c1 = fmaxf(c1, c);
-          }
-        }
+    for (int j = 0; j < NV; ++j) {
+      const int e = e0 + j;
+      const bool in = j < nv && e < a.E;
+      float c = l[j];
+      if (by_score && in) c = (a.sigmoid ? fast_sigmoid(l[j]) : __expf(l[j] - m) * inv) + a.select_bias[e];
+      if (fabsf(c) < INFINITY) cabs = fmaxf(cabs, fabsf(c));
+      key[j] = in ? ((row_nan ? low : order_key(c, low)) & ~PLACE) | (PLACE - j) : 0u;
+    }
+    // Two values closer than tol may be in the other order exactly.  16-bit
+    // logits have no bits where the place goes: their keys are exact.
+    const bool exact_keys = !by_score && (NV == 1 || (sizeof(TX) == 2 && !a.bias));
+    float tol = 0.f;
+    if (!exact_keys || a.top2) {
+      cabs = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(cabs)));
+      tol = 2.f * ((by_score ? eps : 0.f) + KEY_EPS * cabs);
+    }
+    sort_keys<NV>(key);
+    // ---- groups: runs of `lanes` lanes, scored by their first keys
+    if (a.G > 1) {
+      const int lanes = a.per / nv;
+      const int pos = lane % lanes;
+      uint32_t gk;
+      float gtol = tol;
+      if (!a.top2) {
+        uint32_t k1 = key[0] & ~PLACE;
         // after step o a lane covers itself and the min(2 o, rest) - 1 lanes
         // above it inside its group; the group's first lane ends with all
-        const int pos = lane % lanes;
         for (int o = 1; o < lanes; o <<= 1) {
-          const uint32_t ok = __shfl_down_sync(FULL, k1, o);
+          const uint32_t up = __shfl_down_sync(FULL, k1, o);
+          if (pos + o < lanes) k1 = max(k1, up);
+        }
+        gk = __shfl_sync(FULL, k1, min(lane * lanes, 31));  // lane g takes group g's score
+      } else {
+        float c1 = -INFINITY, c2 = -INFINITY;
+        auto value = [&](uint32_t k) {
+          if ((k & ~PLACE) <= low) return -INFINITY;
+          if ((k & ~PLACE) <= KEY_NEG_INF) return 0.f;  // the score of a logit of -inf
+          const float v = key_value(k & ~PLACE);
+          return by_score ? v : a.sigmoid ? fast_sigmoid(v) : __expf(v - m) * inv;
+        };
+        c1 = value(key[0]);
+        if (NV > 1) c2 = value(key[NV > 1 ? 1 : 0]);
+        for (int o = 1; o < lanes; o <<= 1) {
           const float o1 = __shfl_down_sync(FULL, c1, o), o2 = __shfl_down_sync(FULL, c2, o);
-          if (pos + o < lanes && lane + o < 32) {
-            k1 = max(k1, ok);
+          if (pos + o < lanes) {
             c2 = fmaxf(fmaxf(c2, o2), fminf(c1, o1));
             c1 = fmaxf(c1, o1);
           }
         }
-        // lane g takes group g's score
         const int src = min(lane * lanes, 31);
-        k1 = __shfl_sync(FULL, k1, src);
-        c1 = __shfl_sync(FULL, c1, src);
-        c2 = __shfl_sync(FULL, c2, src);
-        const uint32_t gk = a.top2 ? order_key(c1 + c2, KEY_NEG_INF) : k1;
-        int before = 0;
-        for (int g = 0; g < a.G; ++g) {
-          const uint32_t o = __shfl_sync(FULL, gk, g);
-          before += (o > gk || (o == gk && g < lane)) ? 1 : 0;
-        }
-        const bool stays = lane < a.G && before < a.keep;
-        const unsigned kept = __ballot_sync(FULL, stays);
-        if (group_by_score && a.keep < a.G) {
-          const uint32_t in = __reduce_min_sync(FULL, stays ? gk : 0xffffffffu);
-          const uint32_t out = __reduce_max_sync(FULL, !stays && lane < a.G ? gk : 0u);
-          if (out > KEY_NEG_INF && key_value(in) - key_value(out) <= gtol) exact = true;
-        }
-        if (!(kept >> min(lane / lanes, 31) & 1u)) {
-#pragma unroll
-          for (int j = 0; j < NV; ++j) key[j] = min(key[j], low);
-        }
+        const float top = __shfl_sync(FULL, c1, src) + __shfl_sync(FULL, c2, src);
+        gk = order_key(top, KEY_NEG_INF);
+        // a score from a key's logit moves by at most its logit's own error
+        gtol = by_score ? 2.f * tol + 0x1p-22f * cabs
+                        : 4.f * (eps + KEY_EPS * cabs * (a.sigmoid ? 0.25f : inv)) + 0x1p-22f * (a.sigmoid ? 1.f : inv);
       }
-      // ---- K choices, and one more that only shows its distance
-      uint32_t mine = 0u, last = 0u;
+      int before = 0;
+      for (int g = 0; g < a.G; ++g) {
+        const uint32_t o = __shfl_sync(FULL, gk, g);
+        before += (o > gk || (o == gk && g < lane)) ? 1 : 0;
+      }
+      const bool stays = lane < a.G && before < a.keep;
+      const unsigned kept = __ballot_sync(FULL, stays);
+      if (a.keep < a.G && !(exact_keys && !a.top2)) {
+        const uint32_t in = __reduce_min_sync(FULL, stays ? gk : 0xffffffffu);
+        const uint32_t out = __reduce_max_sync(FULL, !stays && lane < a.G ? gk : 0u);
+        if (out > KEY_NEG_INF && key_value(in) - key_value(out) <= gtol) exact = true;
+      }
+      if (!(kept >> min(lane / lanes, 31) & 1u)) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) mine = max(mine, key[j]);
-      const int rounds = by_score ? min(a.K + 1, a.E) : a.K;
-      for (int k = 0; k < rounds && !exact; ++k) {
-        const uint32_t best = __reduce_max_sync(FULL, mine);
-        if (by_score) {
-          if (k > 0 && best > KEY_NEG_INF && key_value(last) - key_value(best) <= tol) exact = true;
-          last = best;
-          if (k == a.K) break;
-        }
-        const int owner = __ffs(__ballot_sync(FULL, mine == best)) - 1;
-        int at = 0;
-        float sv = 0.f;
-        if (lane == owner) {
-          mine = 0u;
-          bool found = false;
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            if (!found && key[j] == best) {
-              found = true;
-              at = e0 + j;
-              sv = s[j];
-              key[j] = 0u;
-            }
-            mine = max(mine, key[j]);
-          }
-        }
-        at = __shfl_sync(FULL, at, owner);
-        sv = __shfl_sync(FULL, sv, owner);
-        if (lane == k) {
-          my_id = at;
-          my_s = sv;
-        }
+        for (int j = 0; j < NV; ++j) key[j] = j < nv && e0 + j < a.E ? low | (PLACE - j) : 0u;
       }
     }
-    if (exact) route_exact<TX>(a, t, s_exact + warp * a.E, &my_id, &my_s);
-    // ---- weights
-    float w = my_s;
-    if (a.renormalize) {
-      float sum = 0.f;
-      for (int k = 0; k < a.K; ++k) sum += __shfl_sync(FULL, my_s, k);
-      w = my_s / (sum < 1e-20f ? 1e-20f : sum);
+    // ---- K picks, and on to the first gap that is certain
+    int n = 0;
+    bool unsure = false, open = false;  // open: this lane's candidate is neither masked nor closed
+    uint32_t last = 0u;
+    while (!exact) {
+      const uint32_t mine = key[0] & ~PLACE;
+      const uint32_t best = __reduce_max_sync(FULL, mine);
+      if (n > 0) {
+        const bool close = !exact_keys && best > KEY_NEG_INF && key_value(last) - key_value(best) <= tol;
+        if (n >= a.K && !close) break;
+        unsure |= close;
+      }
+      if (n == 32) {  // more than a warp of candidates in a row
+        exact = true;
+        break;
+      }
+      const unsigned holders = __ballot_sync(FULL, key[0] != 0u && mine == best);
+      if (holders == 0u) break;  // every expert is picked
+      last = best;
+      const int owner = __ffs(holders) - 1;
+      const int at = owner * nv + (int)(PLACE - (__shfl_sync(FULL, key[0], owner) & PLACE));
+      if (lane == n) {
+        my_id = at;
+        open = best > low;
+      }
+      if (lane == owner) {
+#pragma unroll
+        for (int j = 0; j + 1 < NV; ++j) key[j] = key[j + 1];
+        key[NV - 1] = 0u;
+      }
+      ++n;
     }
-    if (lane < a.K) {
-      a.topk_w[t * a.K + lane] = w * a.scale;
-      if (a.ids32) a.ids32[t * a.K + lane] = my_id;
-      if (a.ids64) a.ids64[t * a.K + lane] = my_id;
+    if (unsure && !exact) {  // lane i: the exact value of candidate i, and its place among the n
+      const float lc = lane < n ? logit_of<TX>(a, t, my_id) : 0.f;
+      double v = lc;
+      if (by_score) {
+        double total = 1.0;
+        if (!a.sigmoid) {
+          total = 0.0;
+          for (int e = lane; e < a.E; e += 32) total += exp((double)logit_of<TX>(a, t, e) - (double)m);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+        }
+        v = (a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)m) / total) + (lane < n ? (double)a.select_bias[my_id] : 0.0);
+      }
+      const double ninf = -(double)INFINITY;
+      v = !open ? ninf : by_score ? v : fmax(v, -1e300);  // a logit of -inf comes before what is masked
+      int rank = 0;
+      for (int j = 0; j < n; ++j) {
+        const double o = __shfl_sync(FULL, v, j);
+        const int oi = __shfl_sync(FULL, my_id, j);
+        rank += (o > v || (o == v && oi < my_id)) ? 1 : 0;
+      }
+      int sorted = 0;
+      for (int j = 0; j < n; ++j) {
+        const int r = __shfl_sync(FULL, rank, j), oi = __shfl_sync(FULL, my_id, j);
+        if (lane == r) sorted = oi;
+      }
+      my_id = sorted;
     }
+    if (!exact && lane < a.K) {  // the scores of the chosen, from their logits
+      const float lc = logit_of<TX>(a, t, my_id);
+      my_s = a.sigmoid ? 1.0f / (1.0f + expf(-lc)) : expf(lc - m) / sum;
+    }
+  }
+  if (exact) route_exact<TX>(a, t, s_exact + warp * a.E, &my_id, &my_s);
+  // ---- weights
+  float w = my_s;
+  if (a.renormalize) {
+    float total = 0.f;
+    for (int k = 0; k < a.K; ++k) total += __shfl_sync(FULL, my_s, k);
+    w = my_s / (total < 1e-20f ? 1e-20f : total);
+  }
+  if (lane < a.K) {
+    a.topk_w[t * a.K + lane] = w * a.scale;
+    if (a.ids32) a.ids32[t * a.K + lane] = my_id;
+    if (a.ids64) a.ids64[t * a.K + lane] = my_id;
   }
 }
 
 template <int NV, typename TX>
 int launch_nv(const GroupedArgs &a, cudaStream_t st) {
-  const int64_t blocks = std::min<int64_t>((a.T + GR_WARPS - 1) / GR_WARPS, (int64_t)rf::num_sms() * 16);
-  // fp64 scratch only where a token can need it: 32 KB at most (E <= 1024)
-  const bool may_be_exact = a.nv == 0 || a.select_bias || (a.top2 && a.G > 1);
-  const size_t smem = may_be_exact ? (size_t)GR_WARPS * a.E * sizeof(double) : 0;
-  router_grouped_kernel<NV, TX><<<(int)blocks, GR_THREADS, smem, st>>>(a);
+  const int64_t blocks = (a.T + GR_WARPS - 1) / GR_WARPS;
+  // fp64 scratch: 32 KB at most (E <= 1024)
+  const size_t smem = (size_t)GR_WARPS * a.E * sizeof(double);
+  router_grouped_kernel<NV, TX><<<(unsigned)blocks, GR_THREADS, smem, st>>>(a);
   return rf::check_launch("rf_moe_router_grouped_topk(selection)");
 }
 
@@ -432,7 +478,7 @@ extern "C" int rf_moe_router_grouped_topk(const void *x, int x_dtype, const void
                "rf_moe_router_grouped_topk: unknown scoring");
   RF_CHECK_ARG(group_score == RF_GROUP_MAX || group_score == RF_GROUP_TOP2,
                "rf_moe_router_grouped_topk: unknown group_score");
-  RF_CHECK_ARG(T >= 0 && H > 0 && E > 0, "rf_moe_router_grouped_topk: sizes must be positive");
+  RF_CHECK_ARG(T >= 0 && T <= 0x7fffffff && H > 0 && E > 0, "rf_moe_router_grouped_topk: sizes must be positive");
   RF_CHECK_ARG(E <= rf::ROUTER_EMAX, "rf_moe_router_grouped_topk: at most 1024 experts");
   RF_CHECK_ARG(num_groups >= 1 && num_groups <= 32 && E % num_groups == 0,
                "rf_moe_router_grouped_topk: num_groups must be 1..32 and divide the experts");

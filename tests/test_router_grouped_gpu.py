@@ -13,8 +13,9 @@ from reframework_b200.moe import grouped_topk
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
-# a score: expf within 2 ulp above and below the fraction (8 half-ulps), their arguments' rounding (12 each, for
-# |l - max| <= 12), up to 37 additions, a division: 70; the renormalising quotient doubles it and adds 16 + 3
+# a score: an accurate exponential (2 ulp) over a sum of fast ones (each within 2 + 1.173 |l - max| ulp, 16 for
+# |l - max| <= 12), the arguments' rounding (12 half ulps each), up to 37 additions, a division:
+# 4 + 32 + 24 + 37 + 1 = 98 roundings; renormalised, the sum cancels: 2 * (4 + 12 + 1) and 16 + 3 more
 W_TOL = 160 * 2.0 ** -24
 
 

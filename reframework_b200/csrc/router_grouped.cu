@@ -174,37 +174,6 @@ __device__ __noinline__ void route_exact(const GroupedArgs &a, int64_t t, double
   *my_s = lane < a.K ? (float)score_of((double)logit_of<TX>(a, t, id)) : 0.f;
 }
 
-// nv consecutive logits from element e0 of row t.
-template <int NV, typename TX>
-__device__ __forceinline__ void load_logits(const GroupedArgs &a, int64_t t, int e0, int nv, float (&l)[NV]) {
-  constexpr int V = 16 / sizeof(TX);
-  if constexpr (NV >= V) {
-    // whole 16-byte vectors: uniform over the launch
-    if (!a.partial && nv == NV && a.E % V == 0) {
-      const TX *row = reinterpret_cast<const TX *>(a.x) + t * a.E + e0;
-#pragma unroll
-      for (int j = 0; j < NV; j += V) {
-        if (e0 + j < a.E) rf::unpack16<TX>(__ldg(reinterpret_cast<const uint4 *>(row + j)), l + j);
-      }
-      if (a.round_dtype >= 0 || a.bias) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (e0 + j >= a.E) continue;
-          if (a.round_dtype >= 0) l[j] = rf::round_dt(a.round_dtype, l[j]);
-          if (a.bias) {
-            l[j] += a.bias[e0 + j];
-            if (a.round_dtype >= 0) l[j] = rf::round_dt(a.round_dtype, l[j]);
-          }
-        }
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (j < nv && e0 + j < a.E) l[j] = logit_of<TX>(a, t, e0 + j);
-}
-
 // Descending, NV a power of two (bitonic: every comparison a min and a max).
 template <int NV>
 __device__ __forceinline__ void sort_keys(uint32_t (&k)[NV]) {
@@ -229,12 +198,47 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[NV]) {
 // adds 2 and the sum half an ulp.
 __device__ __forceinline__ float fast_sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
 
-template <int NV, typename TX>
+// n candidates, one per lane (the first n_open of them neither masked nor
+// closed), in the order of their exact values; returns the id of this lane's place.
+template <typename TX>
+__device__ __noinline__ int settle(const GroupedArgs &a, int64_t t, int id, int n, int n_open, float m) {
+  const int lane = threadIdx.x & 31;
+  const double ninf = -(double)INFINITY;
+  double v = lane < n ? (double)logit_of<TX>(a, t, id) : 0.0;
+  if (a.select_bias) {
+    double total = 1.0;
+    if (!a.sigmoid) {
+      total = 0.0;
+      for (int e = lane; e < a.E; e += 32) total += exp((double)logit_of<TX>(a, t, e) - (double)m);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+    }
+    v = (a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)m) / total) + (lane < n ? (double)a.select_bias[id] : 0.0);
+  }
+  v = lane >= n_open ? ninf : a.select_bias ? v : fmax(v, -1e300);  // a logit of -inf comes before what is masked
+  int rank = 0;
+  for (int j = 0; j < n; ++j) {
+    const double o = __shfl_sync(FULL, v, j);
+    const int oi = __shfl_sync(FULL, id, j);
+    rank += (o > v || (o == v && oi < id)) ? 1 : 0;
+  }
+  int mine = 0;
+  for (int j = 0; j < n; ++j) {
+    const int r = __shfl_sync(FULL, rank, j), oi = __shfl_sync(FULL, id, j);
+    if (lane == r) mine = oi;
+  }
+  return mine;
+}
+
+// WHOLE: every lane's nv experts are NV or none (nv == NV, E a multiple of NV),
+// read as 16-byte vectors where the type has that many.
+template <int NV, typename TX, bool WHOLE>
 __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const GroupedArgs a) {
   extern __shared__ double s_exact[];  // [GR_WARPS][E], for route_exact
   constexpr uint32_t PLACE = NV - 1;   // the low bits of a key: NV - 1 - place in the lane
+  constexpr int V = 16 / sizeof(TX);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int nv = a.nv;
+  const int nv = WHOLE ? NV : a.nv;
   const int e0 = lane * nv;
   const bool by_score = a.select_bias != nullptr;  // else experts are compared by their logits
   const uint32_t low = (by_score ? KEY_NEG_INF : KEY_MASKED) & ~PLACE;
@@ -246,15 +250,36 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
   }
   if (a.logits_out)
     for (int e = lane; e < a.E; e += 32) a.logits_out[t * a.E + e] = logit_of<TX>(a, t, e);
+  auto inside = [&](int j) { return WHOLE ? e0 < a.E : j < nv && e0 + j < a.E; };
   int my_id = 0;
   float my_s = 0.f;
-  bool exact = nv == 0;  // every decision of this token in fp64
+  bool exact = a.nv == 0;  // every decision of this token in fp64
   float m = 0.f, sum = 1.f;  // softmax: the largest logit, the sum
   if (!exact) {
     float l[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) l[j] = -INFINITY;
-    load_logits<NV, TX>(a, t, e0, nv, l);
+    if (WHOLE && NV >= V && !a.partial) {
+      if (e0 < a.E) {
+        const TX *row = reinterpret_cast<const TX *>(a.x) + t * a.E + e0;
+#pragma unroll
+        for (int j = 0; j + V <= NV; j += V) rf::unpack16<TX>(__ldg(reinterpret_cast<const uint4 *>(row + j)), l + j);
+        if (a.round_dtype >= 0 || a.bias) {
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            if (a.round_dtype >= 0) l[j] = rf::round_dt(a.round_dtype, l[j]);
+            if (a.bias) {
+              l[j] += a.bias[e0 + j];
+              if (a.round_dtype >= 0) l[j] = rf::round_dt(a.round_dtype, l[j]);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (inside(j)) l[j] = logit_of<TX>(a, t, e0 + j);
+    }
     bool row_nan = false;
     if (!a.sigmoid) {
       m = l[0];
@@ -264,37 +289,48 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
       sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) sum += j < nv && e0 + j < a.E ? __expf(l[j] - m) : 0.f;
+      for (int j = 0; j < NV; ++j) sum += inside(j) ? __expf(l[j] - m) : 0.f;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
       row_nan = !(sum == sum);
     }
-    // Errors, absolute: of a score (softmax: __expf within 2 + 1.173 |l - m| ulp
+    // Errors: of a score, absolute (softmax: __expf within 2 + 1.173 |l - m| ulp
     // and its argument's rounding, worth 3 ulp of the largest score; the sum's,
-    // with |l - m| at most 8 on average, and its NV + 5 additions; a product),
-    // of c's own rounding, and of the place bits in a key.
+    // with |l - m| at most 8 on average, and its NV + 5 additions; a product);
+    // of a key, relative to its value (a rounding, and the place bits).
     const float inv = 1.0f / sum;
     const float eps = a.sigmoid ? 7.f * 0x1p-24f : (NV + 48) * 0x1p-24f * inv;
-    constexpr float KEY_EPS = (NV > 1 ? 2 * NV : 1) * 0x1p-24f;  // relative, with a rounding
-    // ---- keys
-    uint32_t key[NV];
-    float cabs = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e = e0 + j;
-      const bool in = j < nv && e < a.E;
-      float c = l[j];
-      if (by_score && in) c = (a.sigmoid ? fast_sigmoid(l[j]) : __expf(l[j] - m) * inv) + a.select_bias[e];
-      if (fabsf(c) < INFINITY) cabs = fmaxf(cabs, fabsf(c));
-      key[j] = in ? ((row_nan ? low : order_key(c, low)) & ~PLACE) | (PLACE - j) : 0u;
-    }
-    // Two values closer than tol may be in the other order exactly.  16-bit
-    // logits have no bits where the place goes: their keys are exact.
+    constexpr float KEY_EPS = (NV > 1 ? 2 * NV : 1) * 0x1p-24f;
+    // 16-bit logits have no bits where the place goes: their keys are exact
     const bool exact_keys = !by_score && (NV == 1 || (sizeof(TX) == 2 && !a.bias));
-    float tol = 0.f;
-    if (!exact_keys || a.top2) {
-      cabs = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(cabs)));
-      tol = 2.f * ((by_score ? eps : 0.f) + KEY_EPS * cabs);
+    // Two values no further apart than this may be in the other order exactly.
+    const float tol0 = by_score ? 2.f * eps : 0.f, tol1 = exact_keys ? 0.f : 2.f * KEY_EPS;
+    auto tolerance = [&](float u, float v) { return fmaf(tol1, fmaxf(fabsf(u), fabsf(v)), tol0); };
+    // ---- keys
+    if (by_score) {
+      float sb[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) sb[j] = 0.f;
+      if (WHOLE && NV >= 4 && ((uintptr_t)a.select_bias & 15) == 0) {
+        if (e0 < a.E) {
+#pragma unroll
+          for (int j = 0; j + 4 <= NV; j += 4)
+            rf::unpack16<float>(__ldg(reinterpret_cast<const uint4 *>(a.select_bias + e0 + j)), sb + j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (inside(j)) sb[j] = a.select_bias[e0 + j];
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) l[j] = (a.sigmoid ? fast_sigmoid(l[j]) : __expf(l[j] - m) * inv) + sb[j];
+    }
+    uint32_t key[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) key[j] = inside(j) ? (order_key(l[j], low) & ~PLACE) | (PLACE - j) : 0u;
+    if (row_nan) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) key[j] = inside(j) ? low | (PLACE - j) : 0u;
     }
     sort_keys<NV>(key);
     // ---- groups: runs of `lanes` lanes, scored by their first keys
@@ -302,7 +338,7 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
       const int lanes = a.per / nv;
       const int pos = lane % lanes;
       uint32_t gk;
-      float gtol = tol;
+      float gtol = 0.f;  // top-2 scores
       if (!a.top2) {
         uint32_t k1 = key[0] & ~PLACE;
         // after step o a lane covers itself and the min(2 o, rest) - 1 lanes
@@ -313,15 +349,18 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
         }
         gk = __shfl_sync(FULL, k1, min(lane * lanes, 31));  // lane g takes group g's score
       } else {
+        // l holds the selection scores, or the logits, whose two largest give the scores
         float c1 = -INFINITY, c2 = -INFINITY;
-        auto value = [&](uint32_t k) {
-          if ((k & ~PLACE) <= low) return -INFINITY;
-          if ((k & ~PLACE) <= KEY_NEG_INF) return 0.f;  // the score of a logit of -inf
-          const float v = key_value(k & ~PLACE);
-          return by_score ? v : a.sigmoid ? fast_sigmoid(v) : __expf(v - m) * inv;
-        };
-        c1 = value(key[0]);
-        if (NV > 1) c2 = value(key[NV > 1 ? 1 : 0]);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const float c = l[j] == l[j] && !row_nan ? l[j] : -INFINITY;
+          c2 = fmaxf(c2, fminf(c1, c));
+          c1 = fmaxf(c1, c);
+        }
+        if (!by_score) {  // past the lane's own experts, and for NaN: -inf, a logit of -inf: 0
+          c1 = key[0] >= low + NV ? a.sigmoid ? fast_sigmoid(c1) : __expf(c1 - m) * inv : -INFINITY;
+          c2 = NV > 1 && key[NV > 1 ? 1 : 0] >= low + NV ? a.sigmoid ? fast_sigmoid(c2) : __expf(c2 - m) * inv : -INFINITY;
+        }
         for (int o = 1; o < lanes; o <<= 1) {
           const float o1 = __shfl_down_sync(FULL, c1, o), o2 = __shfl_down_sync(FULL, c2, o);
           if (pos + o < lanes) {
@@ -330,11 +369,14 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
           }
         }
         const int src = min(lane * lanes, 31);
-        const float top = __shfl_sync(FULL, c1, src) + __shfl_sync(FULL, c2, src);
-        gk = order_key(top, KEY_NEG_INF);
-        // a score from a key's logit moves by at most its logit's own error
-        gtol = by_score ? 2.f * tol + 0x1p-22f * cabs
-                        : 4.f * (eps + KEY_EPS * cabs * (a.sigmoid ? 0.25f : inv)) + 0x1p-22f * (a.sigmoid ? 1.f : inv);
+        c1 = __shfl_sync(FULL, c1, src);
+        c2 = __shfl_sync(FULL, c2, src);
+        gk = order_key(c1 + c2, KEY_NEG_INF);
+        // twice a score's error for each of two sums, and roundings of values up to big
+        float big = fabsf(c1) < INFINITY ? fabsf(c1) : 0.f;
+        if (fabsf(c2) < INFINITY) big = fmaxf(big, fabsf(c2));
+        big = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(lane < a.G ? big : 0.f)));
+        gtol = 4.f * eps + 0x1p-21f * big;
       }
       int before = 0;
       for (int g = 0; g < a.G; ++g) {
@@ -346,73 +388,43 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
       if (a.keep < a.G && !(exact_keys && !a.top2)) {
         const uint32_t in = __reduce_min_sync(FULL, stays ? gk : 0xffffffffu);
         const uint32_t out = __reduce_max_sync(FULL, !stays && lane < a.G ? gk : 0u);
-        if (out > KEY_NEG_INF && key_value(in) - key_value(out) <= gtol) exact = true;
+        const float vi = key_value(in), vo = key_value(out);
+        if (out > KEY_NEG_INF && vi - vo <= (a.top2 ? gtol : tolerance(vi, vo))) exact = true;
       }
       if (!(kept >> min(lane / lanes, 31) & 1u)) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) key[j] = j < nv && e0 + j < a.E ? low | (PLACE - j) : 0u;
+        for (int j = 0; j < NV; ++j) key[j] = inside(j) ? low | (PLACE - j) : 0u;
       }
     }
     // ---- K picks, and on to the first gap that is certain
-    int n = 0;
-    bool unsure = false, open = false;  // open: this lane's candidate is neither masked nor closed
-    uint32_t last = 0u;
+    int n = 0, n_open = 0;
+    bool unsure = false;
+    float last = INFINITY;
     while (!exact) {
       const uint32_t mine = key[0] & ~PLACE;
       const uint32_t best = __reduce_max_sync(FULL, mine);
-      if (n > 0) {
-        const bool close = !exact_keys && best > KEY_NEG_INF && key_value(last) - key_value(best) <= tol;
-        if (n >= a.K && !close) break;
-        unsure |= close;
-      }
-      if (n == 32) {  // more than a warp of candidates in a row
-        exact = true;
+      const float v = key_value(best);
+      // (the first gap is infinite, one down to a masked or closed expert NaN or infinite)
+      const bool close = !exact_keys && last - v <= tolerance(last, v) && n > 0 && best > KEY_NEG_INF;
+      if (n >= a.K && (!close || n == 32)) {
+        exact = close;  // more than a warp of candidates in a row
         break;
       }
-      const unsigned holders = __ballot_sync(FULL, key[0] != 0u && mine == best);
+      const unsigned holders = __ballot_sync(FULL, mine == best && key[0] != 0u);
       if (holders == 0u) break;  // every expert is picked
-      last = best;
+      unsure |= close;
+      last = v;
+      n_open += best > low ? 1 : 0;
       const int owner = __ffs(holders) - 1;
-      const int at = owner * nv + (int)(PLACE - (__shfl_sync(FULL, key[0], owner) & PLACE));
-      if (lane == n) {
-        my_id = at;
-        open = best > low;
-      }
-      if (lane == owner) {
+      const int at = owner * nv + (int)(~__shfl_sync(FULL, key[0], owner) & PLACE);
+      if (lane == n) my_id = at;
+      const bool pop = lane == owner;
 #pragma unroll
-        for (int j = 0; j + 1 < NV; ++j) key[j] = key[j + 1];
-        key[NV - 1] = 0u;
-      }
+      for (int j = 0; j + 1 < NV; ++j) key[j] = pop ? key[j + 1] : key[j];
+      key[NV - 1] = pop ? 0u : key[NV - 1];
       ++n;
     }
-    if (unsure && !exact) {  // lane i: the exact value of candidate i, and its place among the n
-      const float lc = lane < n ? logit_of<TX>(a, t, my_id) : 0.f;
-      double v = lc;
-      if (by_score) {
-        double total = 1.0;
-        if (!a.sigmoid) {
-          total = 0.0;
-          for (int e = lane; e < a.E; e += 32) total += exp((double)logit_of<TX>(a, t, e) - (double)m);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-        }
-        v = (a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)m) / total) + (lane < n ? (double)a.select_bias[my_id] : 0.0);
-      }
-      const double ninf = -(double)INFINITY;
-      v = !open ? ninf : by_score ? v : fmax(v, -1e300);  // a logit of -inf comes before what is masked
-      int rank = 0;
-      for (int j = 0; j < n; ++j) {
-        const double o = __shfl_sync(FULL, v, j);
-        const int oi = __shfl_sync(FULL, my_id, j);
-        rank += (o > v || (o == v && oi < my_id)) ? 1 : 0;
-      }
-      int sorted = 0;
-      for (int j = 0; j < n; ++j) {
-        const int r = __shfl_sync(FULL, rank, j), oi = __shfl_sync(FULL, my_id, j);
-        if (lane == r) sorted = oi;
-      }
-      my_id = sorted;
-    }
+    if (unsure && !exact) my_id = settle<TX>(a, t, my_id, n, n_open, m);
     if (!exact && lane < a.K) {  // the scores of the chosen, from their logits
       const float lc = logit_of<TX>(a, t, my_id);
       my_s = a.sigmoid ? 1.0f / (1.0f + expf(-lc)) : expf(lc - m) / sum;
@@ -420,10 +432,12 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
   }
   if (exact) route_exact<TX>(a, t, s_exact + warp * a.E, &my_id, &my_s);
   // ---- weights
+  if (lane >= a.K) my_s = 0.f;
   float w = my_s;
   if (a.renormalize) {
-    float total = 0.f;
-    for (int k = 0; k < a.K; ++k) total += __shfl_sync(FULL, my_s, k);
+    float total = my_s;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);  // K <= 16
     w = my_s / (total < 1e-20f ? 1e-20f : total);
   }
   if (lane < a.K) {
@@ -438,7 +452,8 @@ int launch_nv(const GroupedArgs &a, cudaStream_t st) {
   const int64_t blocks = (a.T + GR_WARPS - 1) / GR_WARPS;
   // fp64 scratch: 32 KB at most (E <= 1024)
   const size_t smem = (size_t)GR_WARPS * a.E * sizeof(double);
-  router_grouped_kernel<NV, TX><<<(unsigned)blocks, GR_THREADS, smem, st>>>(a);
+  if (a.nv == NV && a.E % NV == 0) router_grouped_kernel<NV, TX, true><<<(unsigned)blocks, GR_THREADS, smem, st>>>(a);
+  else router_grouped_kernel<NV, TX, false><<<(unsigned)blocks, GR_THREADS, smem, st>>>(a);
   return rf::check_launch("rf_moe_router_grouped_topk(selection)");
 }
 

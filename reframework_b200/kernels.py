@@ -8,7 +8,6 @@ case raises :class:`reframework_b200._lib.RfMoeError`.
 
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -35,9 +34,15 @@ def _require_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device for a launch (nothing to do when it is)."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(fn, what: str, dev: torch.device, args: tuple) -> None:
+    """``fn(*args, stream)`` on the current stream of ``dev``, which need not be the current device."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream_of(dev))
+    if rc:
+        check(rc, what)
 
 
 def _f32_vector(t: Optional[torch.Tensor], n: int, dev: torch.device, what: str) -> Optional[torch.Tensor]:
@@ -112,45 +117,48 @@ def router_grouped_topk(x: torch.Tensor, gate: Optional[torch.Tensor], top_k: in
     Returns what :func:`router_topk` returns: ``(weights fp32 [T,K], ids32 or None, ids64 or None,
     logits or None, shared_scale or None)``.
     """
+    # the launch is a few microseconds: so is this function, kept to plain calls
     dev = _require_cuda(x, gate, bias, select_bias, shared_gate)
-    if scoring not in _lib.SCORINGS:
+    score, group = _lib.SCORINGS.get(scoring), _lib.GROUP_SCORES.get(group_score)
+    if score is None:
         raise ValueError(f"unknown scoring {scoring!r}; known: {tuple(_lib.SCORINGS)}")
-    if group_score not in _lib.GROUP_SCORES:
+    if group is None:
         raise ValueError(f"unknown group score {group_score!r}; known: {tuple(_lib.GROUP_SCORES)}")
     if x.dim() != 2:
         raise _lib.RfMoeError(f"router_grouped_topk: x must be [T, H] (or [T, E] logits), got {tuple(x.shape)}")
     x = _aligned16(x)
     T, H = x.shape
     E = H
+    xdt = gdt = dtype_code(x.dtype)
+    gate_ptr = sg_ptr = ss = ss_ptr = ws_ptr = None
+    ws_bytes = 0
+    L = lib()
     if gate is not None:
         if gate.dim() != 2 or gate.shape[1] != H:
             raise _lib.RfMoeError(f"router_grouped_topk: gate must be [E, {H}], got {tuple(gate.shape)}")
-        gate = gate.contiguous()
-        E = gate.shape[0]
-    bias = _f32_vector(bias, E, dev, "router_grouped_topk: bias")
-    select_bias = _f32_vector(select_bias, E, dev, "router_grouped_topk: select_bias")
-    w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
-    i32 = torch.empty(T, top_k, dtype=torch.int32, device=dev) if ids32 else None
-    i64 = torch.empty(T, top_k, dtype=torch.int64, device=dev) if ids64 else None
-    lg = torch.empty(T, E, dtype=torch.float32, device=dev) if want_logits else None
-    ss = ws = None
-    ws_bytes = 0
-    if gate is not None:
+        gate = _aligned16(gate)
+        E, gdt, gate_ptr = gate.shape[0], dtype_code(gate.dtype), gate.data_ptr()
         if shared_gate is not None:
             if shared_gate.numel() != H:
                 raise _lib.RfMoeError(f"router_grouped_topk: shared_gate must have {H} elements")
             ss = torch.empty(T, dtype=torch.float32, device=dev)
-            shared_gate = shared_gate.to(dtype=gate.dtype).contiguous()
-        ws_bytes = int(lib().rf_moe_router_workspace_size(T, H, E, int(shared_gate is not None)))
+            shared_gate = _aligned16(shared_gate.to(dtype=gate.dtype))
+            sg_ptr, ss_ptr = shared_gate.data_ptr(), ss.data_ptr()
+        ws_bytes = L.rf_moe_router_workspace_size(T, H, E, int(shared_gate is not None))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = lib().rf_moe_router_grouped_topk(
-            ptr(x), dtype_code(x.dtype), ptr(gate), dtype_code(x.dtype if gate is None else gate.dtype), ptr(bias),
-            T, H, E, top_k, _lib.SCORINGS[scoring], ptr(select_bias), num_groups, topk_groups,
-            _lib.GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
-            -1 if round_dtype is None else dtype_code(round_dtype), ptr(shared_gate), ptr(ss), ptr(w), ptr(i32),
-            ptr(i64), ptr(lg), ptr(ws), ws_bytes, stream_of(dev))
-    check(rc, "rf_moe_router_grouped_topk")
+        ws_ptr = ws.data_ptr()
+    elif shared_gate is not None:
+        raise _lib.RfMoeError("router_grouped_topk: shared_gate needs a gate")
+    bias = _f32_vector(bias, E, dev, "router_grouped_topk: bias")
+    select_bias = _f32_vector(select_bias, E, dev, "router_grouped_topk: select_bias")
+    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    i32 = torch.empty((T, top_k), dtype=torch.int32, device=dev) if ids32 else None
+    i64 = torch.empty((T, top_k), dtype=torch.int64, device=dev) if ids64 else None
+    lg = torch.empty((T, E), dtype=torch.float32, device=dev) if want_logits else None
+    args = (x.data_ptr(), xdt, gate_ptr, gdt, ptr(bias), T, H, E, top_k, score, ptr(select_bias), num_groups, topk_groups,
+            group, 1 if renormalize else 0, scale, -1 if round_dtype is None else dtype_code(round_dtype), sg_ptr, ss_ptr,
+            w.data_ptr(), ptr(i32), ptr(i64), ptr(lg), ws_ptr, ws_bytes)
+    _launch(L.rf_moe_router_grouped_topk, "rf_moe_router_grouped_topk", dev, args)
     return w, i32, i64, lg, ss
 
 
@@ -486,10 +494,8 @@ def int4_pack(codes: torch.Tensor, scales: torch.Tensor, *, group_size: int = 12
     if tuple(scales.shape) != (S, N, -(-K // group_size)):
         raise _lib.RfMoeError(f"int4_pack: scales must be {(S, N, -(-K // group_size))}, got {tuple(scales.shape)}")
     codes, scales = codes.contiguous(), scales.contiguous()
-    with _on(dev):
-        rc = lib().rf_moe_int4_pack(ptr(codes), ptr(scales), dtype_code(w.dtype), S, N, K, group_size, int(gated),
-                                    ptr(w.data), ptr(w.scales), stream_of(dev))
-    check(rc, "rf_moe_int4_pack")
+    _launch(lib().rf_moe_int4_pack, "rf_moe_int4_pack", dev,
+            (ptr(codes), ptr(scales), dtype_code(w.dtype), S, N, K, group_size, int(gated), ptr(w.data), ptr(w.scales)))
     return w
 
 
@@ -504,10 +510,9 @@ def int4_quantize(weight: torch.Tensor, *, group_size: int = 128, gated: bool = 
     S, N, K = weight.shape
     w = _int4_empty(S, N, K, group_size, gated, weight.dtype if dtype is None else dtype, dev, "int4_quantize")
     weight = weight.detach().contiguous()
-    with _on(dev):
-        rc = lib().rf_moe_int4_quantize(ptr(weight), dtype_code(weight.dtype), dtype_code(w.dtype), S, N, K, group_size,
-                                        int(gated), ptr(w.data), ptr(w.scales), stream_of(dev))
-    check(rc, "rf_moe_int4_quantize")
+    _launch(lib().rf_moe_int4_quantize, "rf_moe_int4_quantize", dev,
+            (ptr(weight), dtype_code(weight.dtype), dtype_code(w.dtype), S, N, K, group_size, int(gated), ptr(w.data),
+             ptr(w.scales)))
     return w
 
 
@@ -515,10 +520,8 @@ def int4_dequantize(w: Int4Weights) -> torch.Tensor:
     """``w`` as ``[S, N, K]`` in its layer dtype (each value rounded once; exact for :func:`int4_quantize`'s scales)."""
     dev = _require_cuda(w.data, w.scales)
     out = torch.empty(w.slots, w.rows, w.cols, dtype=w.dtype, device=dev)
-    with _on(dev):
-        rc = lib().rf_moe_int4_dequantize(ptr(w.data), ptr(w.scales), dtype_code(w.dtype), w.slots, w.rows, w.cols,
-                                          w.group_size, int(w.gated), ptr(out), stream_of(dev))
-    check(rc, "rf_moe_int4_dequantize")
+    _launch(lib().rf_moe_int4_dequantize, "rf_moe_int4_dequantize", dev,
+            (ptr(w.data), ptr(w.scales), dtype_code(w.dtype), w.slots, w.rows, w.cols, w.group_size, int(w.gated), ptr(out)))
     return out
 
 
@@ -551,16 +554,15 @@ def moe_experts_int4(x: torch.Tensor, w1: Int4Weights, w2: Int4Weights, weights:
             raise _lib.RfMoeError(f"moe_experts_int4: {name} must be contiguous with x's shape and dtype")
     shared_scale = _f32_vector(shared_scale, T, dev, "moe_experts_int4: shared_scale")
     if out is None:
-        out = torch.empty(T, H, dtype=dt, device=dev)
+        out = torch.empty((T, H), dtype=dt, device=dev)
     L = lib()
     ws_bytes = L.rf_moe_int4_experts_workspace_size(T, K, E, H, I)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = L.rf_moe_int4_experts(ptr(x), dtype_code(dt), ptr(w1.data), ptr(w1.scales), w1.group_size, ptr(w2.data),
-                                   ptr(w2.scales), w2.group_size, ptr(weights), ptr(ids32), T, K, E, H, I,
-                                   _lib.ACTIVATIONS[activation], ptr(shared_y), ptr(shared_scale), ptr(residual), ptr(out),
-                                   ptr(ws), ws_bytes, stream_of(dev))
-    check(rc, "rf_moe_int4_experts")
+    _launch(L.rf_moe_int4_experts, "rf_moe_int4_experts", dev,
+            (x.data_ptr(), dtype_code(dt), w1.data.data_ptr(), w1.scales.data_ptr(), w1.group_size, w2.data.data_ptr(),
+             w2.scales.data_ptr(), w2.group_size, weights.data_ptr(), ids32.data_ptr(), T, K, E, H, I,
+             _lib.ACTIVATIONS[activation], ptr(shared_y), ptr(shared_scale), ptr(residual), out.data_ptr(), ws.data_ptr(),
+             ws_bytes))
     return out
 
 
@@ -596,12 +598,10 @@ def add_rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[
     bias = _f32_vector(bias, H, dev, "add_rmsnorm_q8: bias")
     q = scales = None
     if want_q:
-        q = torch.empty(T, H, dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty(T, H // group_size if group_size else 1, dtype=torch.float32, device=dev)
+        q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((T, H // group_size if group_size else 1), dtype=torch.float32, device=dev)
     normed = torch.empty_like(x) if want_normed else None
-    with _on(dev):
-        rc = lib().rf_moe_add_rmsnorm_q8(ptr(x), ptr(residual), T, H, dtype_code(x.dtype), ptr(weight), ptr(bias),
-                                         float(eps), group_size, None if residual is None else ptr(r), ptr(normed),
-                                         ptr(q), ptr(scales), stream_of(dev))
-    check(rc, "rf_moe_add_rmsnorm_q8")
+    _launch(lib().rf_moe_add_rmsnorm_q8, "rf_moe_add_rmsnorm_q8", dev,
+            (x.data_ptr(), ptr(residual), T, H, dtype_code(x.dtype), weight.data_ptr(), ptr(bias), eps, group_size,
+             None if residual is None else r.data_ptr(), ptr(normed), ptr(q), ptr(scales)))
     return NormQ8(q, scales, r, normed)

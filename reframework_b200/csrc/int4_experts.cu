@@ -557,7 +557,7 @@ bool sizes_ok(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
 
 // The CTA-pair kernel from this many rows per expert on (the mean over the
 // experts that can have any: the counts are on the device).
-constexpr int64_t PAIR_ROWS = 8;
+constexpr int64_t PAIR_ROWS = 9;
 
 bool use_pair(int64_t T, int64_t K, int64_t E) {
   const int impl = rf::gemm_impl();

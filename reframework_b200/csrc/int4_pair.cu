@@ -46,8 +46,11 @@ namespace {
 
 constexpr int Q_BK = 64;                        // swizzle atom depth (elements)
 constexpr int Q_KSUB = 2;                       // atoms per stage
+constexpr int Q_TOK = 256;                      // token rows per tile
 constexpr int Q_A_SUB = 128 * Q_BK * 2;         // 16 KB: this CTA's weight rows
+constexpr int Q_B_SUB = (Q_TOK / 2) * Q_BK * 2; // 16 KB: this CTA's token rows
 constexpr int Q_STAGES = 3;
+constexpr int Q_STAGE_BYTES = Q_KSUB * (Q_A_SUB + Q_B_SUB);
 constexpr int Q_EPI_WARPS = 4;
 constexpr int Q_CODE_WARPS = 4;                 // code warps of a stage: 32 weight rows each
 constexpr int Q_COPY_WARP = 2 + Q_EPI_WARPS + Q_STAGES * Q_CODE_WARPS;  // the last warp
@@ -56,30 +59,17 @@ constexpr int Q_BLOCKS = 8;                     // row blocks (16 rows) of a CTA
 constexpr int Q_CODE_BYTES = Q_BLOCKS * Q_KSUB * rf::I4_BLOCK;  // 8 KB
 constexpr int Q_SCALE_BYTES = Q_BLOCKS * 4 * rf::I4_ROWS * 2;   // 1 KB: up to four groups
 constexpr int Q_MAX_E = 1024;
-constexpr int Q_MAX_CODE_SLOTS = 2 * Q_STAGES;
-constexpr int Q_NUM_BARS = 2 * Q_STAGES + 5 + 2 * Q_MAX_CODE_SLOTS;  // full, empty, tmem full x2, tmem empty x2, drain, codes full, codes empty
+constexpr int Q_NUM_BARS = 4 * Q_STAGES + 5;  // full, empty, tmem full x2, tmem empty x2, drain, codes full, codes empty
 constexpr int Q_N_BOXES = 5;                    // token boxes of 8, 16, 32, 64, 128 rows
 constexpr unsigned Q_EPI_SLEEP_NS = 256;
 constexpr uint64_t Q_ABORT_DRAIN_NS = 1000000;  // pause for copies in flight after an abort
 constexpr uint32_t Q_TMEM_COLS = 512;
-
-// The two forms: tiles of 256 tokens with a slot of codes per stage, and tiles
-// of 128 tokens whose smaller token slots leave room for two slots of codes per
-// stage.  A copy of codes takes about 2500 cycles from memory: with one slot
-// that is the cycle of a stage slot when tiles are small (16 tokens: 2670 cycles
-// for three stages), and large tiles hide it behind their MMAs.
-template <int TOK>
-struct PairForm {
-  static constexpr int B_SUB = (TOK / 2) * Q_BK * 2;  // this CTA's token rows
-  static constexpr int CODE_SLOTS = TOK == 256 ? Q_STAGES : 2 * Q_STAGES;
-  static constexpr size_t SMEM_BYTES = 1024 + (size_t)Q_STAGES * Q_KSUB * (Q_A_SUB + B_SUB) +
-                                       (size_t)CODE_SLOTS * (Q_CODE_BYTES + Q_SCALE_BYTES) + Q_NUM_BARS * 8 + 16 +
-                                       (size_t)(Q_MAX_E + 1) * 4;
-  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-  static_assert(B_SUB % 1024 == 0, "swizzle atoms");
-};
+constexpr size_t Q_SMEM_BYTES =
+    1024 + (size_t)Q_STAGES * Q_STAGE_BYTES + (size_t)Q_STAGES * (Q_CODE_BYTES + Q_SCALE_BYTES) + Q_NUM_BARS * 8 + 16 +
+    (size_t)(Q_MAX_E + 1) * 4;
+static_assert(Q_SMEM_BYTES <= 227 * 1024, "shared memory");
 static_assert(Q_CODE_BYTES % 128 == 0 && Q_SCALE_BYTES % 128 == 0, "TMA destinations");
-static_assert(Q_A_SUB % 1024 == 0, "swizzle atoms");
+static_assert(Q_A_SUB % 1024 == 0 && Q_B_SUB % 1024 == 0, "swizzle atoms");
 
 struct PairArgs {
   const int32_t *offsets, *counts;
@@ -177,17 +167,16 @@ __device__ __forceinline__ void store_gated(const uint32_t (&v)[16], int lane, T
 }
 
 // SUBS: scale groups in a stage's 128 k (1, 2 or 4).
-template <typename T, bool GATED, int SUBS, int TOK>
+template <typename T, bool GATED, int SUBS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     int4_pair_gemm(const __grid_constant__ TokMaps tmX, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ CUtensorMap tmS, const PairArgs p) {
-  constexpr int B_SUB = PairForm<TOK>::B_SUB, CODE_SLOTS = PairForm<TOK>::CODE_SLOTS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sA = smem;
   uint8_t *sB = sA + Q_STAGES * Q_KSUB * Q_A_SUB;
-  uint8_t *sQ = sB + Q_STAGES * Q_KSUB * B_SUB;  // [slot] codes, then scales
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sQ + CODE_SLOTS * (Q_CODE_BYTES + Q_SCALE_BYTES));
+  uint8_t *sQ = sB + Q_STAGES * Q_KSUB * Q_B_SUB;  // [slot] codes, then scales
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sQ + Q_STAGES * (Q_CODE_BYTES + Q_SCALE_BYTES));
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Q_NUM_BARS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   int *tile_prefix = reinterpret_cast<int *>(tmem_holder + 4);  // [E+1]
@@ -203,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 #define TEMPTY(a) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 2 + (a)))
   const uint32_t DRAIN = bar0 + 8u * (uint32_t)(2 * Q_STAGES + 4);
 #define CFULL(s) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 5 + (s)))
-#define CEMPTY(s) (bar0 + 8u * (uint32_t)(2 * Q_STAGES + 5 + Q_MAX_CODE_SLOTS + (s)))
+#define CEMPTY(s) (bar0 + 8u * (uint32_t)(3 * Q_STAGES + 5 + (s)))
   const uint32_t peer_abort = mapa_shared(smem_u32((const void *)abort_flag), rank ^ 1u);
 
   // bounded wait with cluster-scope acquire; on expiry both CTAs are told to stop
@@ -229,8 +218,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     for (int s = 0; s < Q_STAGES; ++s) {
       mbar_init(FULL(s), 1 + 2 * Q_CODE_WARPS);  // the first CTA's: its token producer and the pair's code warps
       mbar_init(EMPTY(s), 1);
-    }
-    for (int s = 0; s < CODE_SLOTS; ++s) {
       mbar_init(CFULL(s), 1);
       mbar_init(CEMPTY(s), Q_CODE_WARPS);
     }
@@ -248,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
   }
   if (threadIdx.x == 32)
     for (int i = 0; i < Q_N_BOXES; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX.m[i]) : "memory");
-  for (int e = threadIdx.x; e < E; e += Q_THREADS) tile_prefix[e + 1] = (p.counts[e] + TOK - 1) / TOK * p.n_fb;
+  for (int e = threadIdx.x; e < E; e += Q_THREADS) tile_prefix[e + 1] = (p.counts[e] + Q_TOK - 1) / Q_TOK * p.n_fb;
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_holder), Q_TMEM_COLS);
     tmem_relinquish_pair();
@@ -284,13 +271,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
       else hi = mid - 1;
     }
     const int cnt = __ldg(p.counts + lo);
-    const int ntb = (cnt + TOK - 1) / TOK;
+    const int ntb = (cnt + Q_TOK - 1) / Q_TOK;
     const int local = t - tile_prefix[lo];
     fb = local / ntb;
     const int tb = local - fb * ntb;
     e = lo;
-    row0 = __ldg(p.offsets + lo) + tb * TOK;
-    ntok = min(TOK, cnt - tb * TOK);
+    row0 = __ldg(p.offsets + lo) + tb * Q_TOK;
+    ntok = min(Q_TOK, cnt - tb * Q_TOK);
   };
 
   if (warp == 0) {
@@ -311,11 +298,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         ok = __all_sync(0xffffffffu, pwait(EMPTY(stage), phase ^ 1u, 0));
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t b_dst = smem_u32(sB + stage * Q_KSUB * B_SUB);
+          const uint32_t b_dst = smem_u32(sB + stage * Q_KSUB * Q_B_SUB);
           if (rank == 0) mbar_expect_tx(FULL(stage), 2u * bytes);  // both CTAs load the same box sizes
 #pragma unroll
           for (int j = 0; j < Q_KSUB; ++j)
-            tma_load_2d_pair(b_dst + (uint32_t)(j * B_SUB), &tmX.m[bi], full0 + 8u * (uint32_t)stage,
+            tma_load_2d_pair(b_dst + (uint32_t)(j * Q_B_SUB), &tmX.m[bi], full0 + 8u * (uint32_t)stage,
                              (kb * Q_KSUB + j) * Q_BK, xrow);
         }
         __syncwarp();
@@ -354,13 +341,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t a0 = a_desc + (uint32_t)(stage * (Q_KSUB * Q_A_SUB >> 4));
-          const uint32_t b0 = b_desc + (uint32_t)(stage * (Q_KSUB * B_SUB >> 4));
+          const uint32_t b0 = b_desc + (uint32_t)(stage * (Q_KSUB * Q_B_SUB >> 4));
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < Q_KSUB; ++j)
 #pragma unroll
               for (int k = 0; k < Q_BK / 16; ++k)
-                tc_mma_pair_lo(d, a0 + (uint32_t)((j * Q_A_SUB + k * 32) >> 4), b0 + (uint32_t)((j * B_SUB + k * 32) >> 4),
+                tc_mma_pair_lo(d, a0 + (uint32_t)((j * Q_A_SUB + k * 32) >> 4), b0 + (uint32_t)((j * Q_B_SUB + k * 32) >> 4),
                                idesc, (kb | j | k) ? 1u : 0u);
             tc_commit_both(EMPTY(stage));  // frees the stage in both CTAs once read
             if (kb == num_kb - 1) tc_commit_both(TFULL(acc));
@@ -449,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
           tma_load_2d(sdst + Q_SCALE_BYTES / 2, &tmS, CFULL(stage), kb * (SUBS * rf::I4_ROWS), rb1);
         }
         __syncwarp();
-        if (++stage == CODE_SLOTS) {
+        if (++stage == Q_STAGES) {
           stage = 0;
           phase ^= 1u;
         }
@@ -466,10 +453,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     const int cw = warp - 2 - Q_EPI_WARPS;
     const int slot = cw / Q_CODE_WARPS, j = cw % Q_CODE_WARPS;  // its 32 of the CTA's 128 rows
     const int g = lane >> 2, c = lane & 3;
-    // its codes come through the slots slot, slot + Q_STAGES, ... of their ring in turn
-    uint32_t codes = smem_u32(sQ) + (uint32_t)(slot * (Q_CODE_BYTES + Q_SCALE_BYTES));
-    int cslot = slot;
-    uint32_t cphase = 0;
+    const uint32_t codes = smem_u32(sQ) + (uint32_t)(slot * (Q_CODE_BYTES + Q_SCALE_BYTES));
     const int steps = pair < total ? ((total - 1 - pair) / npairs + 1) * num_kb : 0;
     // rows g and g + 8 of a block, 16-byte pieces 4 h + c of their 128 bytes,
     // swizzled; the first one written has h = g & 1
@@ -478,7 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     const uint32_t full = mapa_shared(FULL(slot), 0);
     uint32_t phase = 0;
     for (int s = slot; s < steps; s += Q_STAGES, phase ^= 1u) {
-      bool ok = __all_sync(0xffffffffu, pwait(CFULL(cslot), cphase, 0));  // the warp leaves together
+      bool ok = __all_sync(0xffffffffu, pwait(CFULL(slot), phase, 0));  // the warp leaves together
       if (!ok) break;
       uint4 q[2][Q_KSUB];
       uint32_t sc[2][SUBS];
@@ -496,15 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
         for (int i = 0; i < SUBS; ++i) sc[r][i] = ld_shared_u32(ss + (uint32_t)(i * 4));
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(CEMPTY(cslot));  // the codes are in registers
-      if (CODE_SLOTS == Q_STAGES || cslot >= Q_STAGES) {
-        cphase ^= 1u;
-        codes -= (uint32_t)((cslot - slot) * (Q_CODE_BYTES + Q_SCALE_BYTES));
-        cslot = slot;
-      } else {
-        cslot += Q_STAGES;
-        codes += (uint32_t)(Q_STAGES * (Q_CODE_BYTES + Q_SCALE_BYTES));
-      }
+      if (lane == 0) mbar_arrive(CEMPTY(slot));  // the codes are in registers
       // 16-bit values of rows g (v[..][0]) and g + 8, before the wait: only
       // the stores stay between a slot's release and its next use
       uint32_t v[2][Q_KSUB][2][2][4];
@@ -564,20 +540,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 #undef TEMPTY
 }
 
-template <typename T, bool GATED, int SUBS, int TOK>
+template <typename T, bool GATED, int SUBS>
 int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
-  auto kern = int4_pair_gemm<T, GATED, SUBS, TOK>;
-  constexpr size_t SMEM = PairForm<TOK>::SMEM_BYTES;
+  auto kern = int4_pair_gemm<T, GATED, SUBS>;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   static int clusters = 0;
   std::call_once(once, [&] {
-    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q_SMEM_BYTES);
     if (err != cudaSuccess) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * std::max(1, rf::num_sms() / 2), 1, 1);
     cfg.blockDim = dim3(Q_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = SMEM;
+    cfg.dynamicSmemBytes = Q_SMEM_BYTES;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2;
@@ -591,26 +566,15 @@ int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &m
     cudaGetLastError();
     return rf::fail(RF_ERR_CUDA, "4-bit products: the CTA-pair kernel does not fit this device");
   }
-  kern<<<2 * clusters, Q_THREADS, SMEM, st>>>(mx, mw, ms, p);
+  kern<<<2 * clusters, Q_THREADS, Q_SMEM_BYTES, st>>>(mx, mw, ms, p);
   return rf::check_launch(GATED ? "4-bit gated products (CTA pairs)" : "4-bit down products (CTA pairs)");
 }
 
-template <typename T, bool GATED, int TOK>
-int launch_pair_g(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
-  if (p.group == 32) return launch_pair_t<T, GATED, 4, TOK>(mx, mw, ms, p, st);
-  if (p.group == 64) return launch_pair_t<T, GATED, 2, TOK>(mx, mw, ms, p, st);
-  return launch_pair_t<T, GATED, 1, TOK>(mx, mw, ms, p, st);
-}
-
-// 256-token tiles where an expert has many rows on average (the counts are on
-// the device; of the experts that can have any).
-constexpr int64_t WIDE_ROWS = 96;
-
 template <typename T, bool GATED>
-int launch_pair_w(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, int64_t rows,
-                  cudaStream_t st) {
-  if (rows >= WIDE_ROWS * std::min<int64_t>(p.E, rows)) return launch_pair_g<T, GATED, 256>(mx, mw, ms, p, st);
-  return launch_pair_g<T, GATED, 128>(mx, mw, ms, p, st);
+int launch_pair_g(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
+  if (p.group == 32) return launch_pair_t<T, GATED, 4>(mx, mw, ms, p, st);
+  if (p.group == 64) return launch_pair_t<T, GATED, 2>(mx, mw, ms, p, st);
+  return launch_pair_t<T, GATED, 1>(mx, mw, ms, p, st);
 }
 
 }  // namespace
@@ -647,10 +611,9 @@ int launch_int4_pair(const Int4Gemm &g, bool gated, cudaStream_t st) {
                         (uint64_t)p.sh.groups * I4_ROWS * 2, scale_cols, 4))
     return rf::fail(RF_ERR_CUDA, "4-bit products: the weights' tensor maps could not be encoded");
   if (g.dtype == RF_F16)
-    return gated ? launch_pair_w<__half, true>(mx, mw, ms, p, g.rows, st)
-                 : launch_pair_w<__half, false>(mx, mw, ms, p, g.rows, st);
-  return gated ? launch_pair_w<__nv_bfloat16, true>(mx, mw, ms, p, g.rows, st)
-               : launch_pair_w<__nv_bfloat16, false>(mx, mw, ms, p, g.rows, st);
+    return gated ? launch_pair_g<__half, true>(mx, mw, ms, p, st) : launch_pair_g<__half, false>(mx, mw, ms, p, st);
+  return gated ? launch_pair_g<__nv_bfloat16, true>(mx, mw, ms, p, st)
+               : launch_pair_g<__nv_bfloat16, false>(mx, mw, ms, p, st);
 }
 
 }  // namespace rf

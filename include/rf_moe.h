@@ -56,6 +56,9 @@
  *                           one kernel
  *   rf_moe_peer_alloc / _open / _close / _free  buffers mapped by every peer
  *                           (no reference counterpart)
+ *   rf_moe_router_grouped_topk, rf_moe_int4_*  (no reference counterpart:
+ *                           grouped routing and 4-bit experts)
+ *   rf_moe_add_rmsnorm_q8   reframework/layers/norm.py:27-53 with an 8-bit output
  *   rf_moe_int8_quantize, rf_moe_int8_grouped_gemm, rf_moe_split_combine
  *                           the int8 half of the CPU/GPU expert split
  *                           (reframework/moe/fused.py:89-197,
@@ -306,7 +309,9 @@ int rf_moe_grouped_gemm_gated_gather(const void *x, int64_t x_rows, const int32_
  * chosen per launch), 1 = CUDA cores only (used by tests to cross-check the
  * two implementations), 2 / 3 / 4 = single-CTA tensor-core kernel with tile
  * width N = 256 / 128 / 64, 5 = the CTA-pair tensor-core kernel (weights on
- * the MMA's M side; the automatic choice for 16-bit layers).
+ * the MMA's M side; the automatic choice for 16-bit layers).  4-bit experts
+ * (rf_moe_int4_experts) run their few-row kernel with 1 (up to 1024 pairs) and
+ * their CTA-pair kernel with 5.
  * No reference counterpart (the reference has a single torch matmul path).
  */
 int rf_moe_set_gemm_impl(int impl);

@@ -20,6 +20,8 @@
 // a gated weight's gate and up halves are padded to whole row blocks each.
 #pragma once
 
+#include <map>
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -86,6 +88,25 @@ template <> __device__ __forceinline__ uint32_t int4_pair<__half>(uint32_t word,
   const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
   return *reinterpret_cast<const uint32_t *>(&v);
 }
+
+// What a kernel's set-up found on each device (function attributes are a
+// device's own): `find` runs once per device, on the current one; 0: it failed.
+class PerDevice {
+ public:
+  template <typename F>
+  int get(F find) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> lock(mu_);
+    auto it = found_.find(dev);
+    if (it == found_.end()) it = found_.emplace(dev, find()).first;
+    return it->second;
+  }
+
+ private:
+  std::mutex mu_;
+  std::map<int, int> found_;
+};
 
 // One grouped product over all experts, rows in permuted order.
 struct Int4Gemm {

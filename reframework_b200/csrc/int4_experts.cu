@@ -7,21 +7,23 @@
 // the second product's 16-bit operand; everything else stays fp32 up to out.
 //
 // Few pairs (T * K <= 1024, few rows per expert): int4_few_kernel, bound by
-// reading the weights, half a byte each, and close behind by the instructions
-// that unpack them.  A block takes 32 weight rows at a time (gated: 16 gate and
-// their 16 up rows) of one expert over the whole reduction, its eight warps an
-// eighth of it each; a lane's 16-byte word of the stored layout is its fragment
-// of four 16 x 16 tiles of mma.sync, the codes as exact 16-bit integers, and
-// the tokens (8 at a time) are read straight from their rows.  A group's
-// sums are scaled in fp32 after its products.  The eight partial sums meet in
-// shared memory in warp order, so results do not depend on timing.  There is no
-// permutation: every block finds its expert's pairs in the ids, h and y rows
-// are the pairs themselves, and the three launches (gated, down, combine) are
-// chained by programmatic dependent launch, each waiting for its predecessor's
-// rows only after its ids and first weights are on the way.
+// reading the weights, half a byte each, and by the instructions that unpack
+// them (about 14 for 256 weights of a warp, of which 7 shift and mask).  A job is
+// 32 weight rows a warp group (gated: 16 gate and their 16 up rows) of one
+// expert over the whole reduction, against 8 of its tokens.  A lane's 16-byte
+// word of the stored layout is its fragment of four 16 x 16 tiles of mma.sync,
+// the codes as exact 16-bit integers; the tokens are read straight from their
+// rows.  A group's sums are scaled in fp32 after its products.  The warps'
+// partial sums meet in shared memory in warp order, so results do not depend on
+// timing.  There is no permutation: every block finds the experts' pairs in the
+// ids, h and y rows are the pairs themselves, and the three launches (gated,
+// down, combine) are chained by programmatic dependent launch, each waiting for
+// its predecessor's rows only after its ids and first weights are on the way.
+// Measured: 7 tokens through eight experts of 4096 x 14336 144 us (73 % of the
+// measured HBM rate), one token 58 us; 64 tokens through 60 experts of 2048 x
+// 1408 85 us, one token 15 us.
 // Many rows per expert: permute with the row gather, then int4_pair.cu.
 #include <algorithm>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -37,7 +39,10 @@ constexpr int FW_THREADS = FW_WARPS * 32;
 constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
 constexpr int FW_STEP = rf::I4_STEP;
 constexpr int FW_AHEAD = 4;     // a power of two: ring slots of a warp: steps of codes on their way, and the one in use
-constexpr int FW_MANY_JOBS = 2368;  // 32-row units from which two warps share a unit's k instead of eight
+// 32-row units from which two warps share a unit's k instead of eight: longer
+// runs per job (64 tokens through 60 experts: 111 -> 101 us), while below it jobs
+// of four units would leave blocks idle.
+constexpr int FW_MANY_JOBS = 2368;
 constexpr int KMAX = 16;
 
 struct FewArgs {
@@ -198,7 +203,10 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
   const int n = sm.active;
   const int64_t jobs = (int64_t)sm.prefix[n] * p.units;
   const int j0 = (int)(jobs * blockIdx.x / gridDim.x), j1 = (int)(jobs * (blockIdx.x + 1) / gridDim.x);
-  if (j0 >= j1) return;
+  if (j0 >= j1) {
+    if (!GATED) wait_for_previous();  // no launch of the chain ends before the one in front of it
+    return;
+  }
   const int steps = (int)p.sh.k_blocks / 2;
   constexpr int RG = FW_WARPS / KS;
   const int rg = warp / KS, ks = warp % KS;
@@ -414,14 +422,13 @@ template <typename T, bool GATED, int SUBS, int KS>
 int launch_few_k(FewArgs p, cudaStream_t st) {
   auto kern = int4_few_kernel<T, GATED, SUBS, KS>;
   const char *what = GATED ? "4-bit gated products (few rows)" : "4-bit down products (few rows)";
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  static int resident = 0;
-  std::call_once(once, [&] {
-    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FewShared));
-    if (err == cudaSuccess) err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, FW_THREADS, sizeof(FewShared));
+  static rf::PerDevice fit;
+  const int resident = fit.get([&]() -> int {
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FewShared)) != cudaSuccess) return 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, FW_THREADS, sizeof(FewShared)) == cudaSuccess ? n : 0;
   });
-  if (err != cudaSuccess || resident < 1) {
+  if (resident < 1) {
     cudaGetLastError();
     return rf::fail(RF_ERR_CUDA, std::string(what) + ": the kernel does not fit this device");
   }
@@ -556,7 +563,10 @@ bool sizes_ok(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I) {
 }
 
 // The CTA-pair kernel from this many rows per expert on (the mean over the
-// experts that can have any: the counts are on the device).
+// experts that can have any: the counts are on the device).  Either side of it,
+// us of few rows / CTA pairs: 60 experts of 2048 x 1408, 6.4 rows 95 / 119, 8.5
+// rows 112 / 119, 12.8 rows 150 / 120; eight of 4096 x 14336, 8 rows 266 / 282,
+// 12 rows 332 / 282; 64 experts, 9.4 rows 129 / 127.
 constexpr int64_t PAIR_ROWS = 9;
 
 bool use_pair(int64_t T, int64_t K, int64_t E) {

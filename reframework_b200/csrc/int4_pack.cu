@@ -13,8 +13,6 @@
 
 #include "int4.cuh"
 
-RF_DEVICE_ERROR_WORD();
-
 namespace {
 
 constexpr int THREADS = 256;

@@ -6,7 +6,7 @@
 // As in gemm_pair.cu the weights are the MMA's M side (128 rows per CTA, 256
 // per pair) and the expert's token rows its N side (up to 256 in steps of 16,
 // half of them in each CTA's shared memory).  The weights arrive as 4-bit codes
-// (int4.cuh): bulk copies bring a CTA's codes and scales into a ring of their
+// (int4.cuh): TMA copies bring a CTA's codes and scales into a ring of their
 // own, and code warps turn each word into eight 16-bit values
 // scale * (code - 8) and write them where a TMA copy would have put 16-bit
 // weights (K-major, 128-byte swizzle).  The product of a code with a scale of
@@ -14,6 +14,15 @@
 // nothing here; a scale with more bits is rounded once per weight, to nearest.
 // Gated tiles put 16 gate rows and their 16 up rows into one quadrant of 32
 // TMEM lanes, so the epilogue pairs them with one shuffle.
+//
+// Bound by the MMAs with tiles of 256 tokens: a stage of 128 k takes 1024 cycles
+// of them (4096 tokens through eight experts of 4096 x 14336: 1.89 ms in all,
+// 95 % of the measured bf16 peak).  With few tokens a stage takes 800-860 cycles
+// whatever their number: 32 KB of 16-bit rows are written to shared memory and
+// read back, 18 KB of codes pass in and out, about 700 cycles of its bandwidth
+// (16 tokens through the same experts: 0.28 ms, 40 % of the time their codes
+// take from memory).  Tried without gain there: a ring of tokens of its own, two
+// slots of codes per stage, 24 code warps, codes called into L2 ahead.
 //
 // Roles (a cluster of two CTAs per pair, persistent, 14 warps):
 //   warp 0        TMA producer of this CTA's token rows
@@ -33,7 +42,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "int4.cuh"
@@ -126,14 +134,6 @@ __device__ __forceinline__ void tc_mma_pair_lo(uint32_t d, uint32_t a_lo, uint32
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SW128_DESC_HI)
       : "memory");
 }
-// Arrive on the barrier at this offset in both CTAs once all MMAs issued so far have completed.
-__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
-      : "memory");
-}
-
 // Two 16-bit products, each rounded to nearest (exact for short scales).
 template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
@@ -276,8 +276,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     fb = local / ntb;
     const int tb = local - fb * ntb;
     e = lo;
-    row0 = __ldg(p.offsets + lo) + tb * Q_TOK;
-    ntok = min(Q_TOK, cnt - tb * Q_TOK);
+    // the rows in equal blocks: 800 rows as 4 x 208 or less, not 3 x 256 and 32
+    const int per = ((cnt + ntb - 1) / ntb + 15) & ~15;  // <= Q_TOK, so the last block has rows
+    row0 = __ldg(p.offsets + lo) + tb * per;
+    ntok = min(per, cnt - tb * per);
   };
 
   if (warp == 0) {
@@ -323,6 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
       // and descriptors stay warp-uniform (inside a one-lane branch an MMA took
       // 88 cycles to issue, most of it moving its operands to uniform registers).
       const uint32_t IDESC = pair_idesc_base<T>();
+      const uint32_t peer_bars = mapa_shared(bar0, 1);
       const uint32_t a_desc = sw128_desc_lo(smem_u32(sA)), b_desc = sw128_desc_lo(smem_u32(sB));
       int stage = 0, it = 0;
       uint32_t phase = 0;
@@ -349,8 +352,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
               for (int k = 0; k < Q_BK / 16; ++k)
                 tc_mma_pair_lo(d, a0 + (uint32_t)((j * Q_A_SUB + k * 32) >> 4), b0 + (uint32_t)((j * Q_B_SUB + k * 32) >> 4),
                                idesc, (kb | j | k) ? 1u : 0u);
-            tc_commit_both(EMPTY(stage));  // frees the stage in both CTAs once read
-            if (kb == num_kb - 1) tc_commit_both(TFULL(acc));
+            tc_commit_pair(EMPTY(stage));  // frees the stage in both CTAs once read
+            tc_commit_pair(peer_bars + (EMPTY(stage) - bar0));
+            if (kb == num_kb - 1) {
+              tc_commit_pair(TFULL(acc));
+              tc_commit_pair(peer_bars + (TFULL(acc) - bar0));
+            }
           }
           __syncwarp();
           if (++stage == Q_STAGES) {
@@ -543,12 +550,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 template <typename T, bool GATED, int SUBS>
 int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
   auto kern = int4_pair_gemm<T, GATED, SUBS>;
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  static int clusters = 0;
-  std::call_once(once, [&] {
-    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q_SMEM_BYTES);
-    if (err != cudaSuccess) return;
+  static rf::PerDevice fit;
+  const int clusters = fit.get([&]() -> int {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q_SMEM_BYTES) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * std::max(1, rf::num_sms() / 2), 1, 1);
     cfg.blockDim = dim3(Q_THREADS, 1, 1);
@@ -560,9 +564,10 @@ int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &m
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    err = cudaOccupancyMaxActiveClusters(&clusters, (void *)kern, &cfg);
+    int n = 0;
+    return cudaOccupancyMaxActiveClusters(&n, (void *)kern, &cfg) == cudaSuccess ? n : 0;
   });
-  if (err != cudaSuccess || clusters < 1) {
+  if (clusters < 1) {
     cudaGetLastError();
     return rf::fail(RF_ERR_CUDA, "4-bit products: the CTA-pair kernel does not fit this device");
   }

@@ -17,8 +17,6 @@
 
 #include "common.cuh"
 
-RF_DEVICE_ERROR_WORD();
-
 namespace {
 
 constexpr float E4M3_MAX = 448.0f;

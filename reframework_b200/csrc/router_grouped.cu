@@ -28,8 +28,6 @@
 // of which 8 sigmoids a lane, a sort of 8 and 9 picks.
 #include "router.cuh"
 
-RF_DEVICE_ERROR_WORD();
-
 namespace {
 
 constexpr int GR_WARPS = 4;

@@ -170,13 +170,13 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile
 // SUBS: scale groups in a step's 128 k (1, 2 or 4).  KS: warps that share a
 // row group's k; the block's 8 / KS row groups are 32 weight rows each.
 //
-// The codes go to the tensor cores as code + B (B = 128 in bf16, 1024 in fp16:
-// a shift and one three-input logic operation per pair), and a group's sums
-// start from -(B + 8) * sum x, itself a product, with a matrix of -(B + 8), that
-// the two row blocks share: sum x (code + B) - (B + 8) sum x = sum x (code - 8).
+// The codes go to the tensor cores as code + B (B = 128 in bf16, 16 in fp16: a
+// shift and one three-input logic operation per pair), and a group's sums start
+// from -(B + 8) * sum x, itself a product, with a matrix of -(B + 8), that the two
+// row blocks share: sum x (code + B) - (B + 8) sum x = sum x (code - 8).
 // Subtracting B + 8 from every code instead took 4 of 15 instructions a word.
-// The larger terms cost at most (B + 16) * 2^-24 of |sum x| in fp32, far below
-// the 16-bit rounding of the result.
+// The larger terms cost at most (2 B + 24) * 2^-24 of sum |x| in fp32, against
+// 16-bit roundings of the result of 2^-8 and 2^-11.
 //
 // Each warp copies its codes into a ring of its own, FW_AHEAD - 1 steps before
 // their use and across the ends of jobs: a job is only a few steps long per
@@ -185,7 +185,7 @@ template <typename T, bool GATED, int SUBS, int KS>
 __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p) {
   extern __shared__ __align__(16) uint8_t few_smem[];
   FewShared &sm = *reinterpret_cast<FewShared *>(few_smem);
-  constexpr uint32_t OFFSET = std::is_same<T, __half>::value ? 0xe408e408u : 0xc308c308u;  // -1032, -136 twice
+  constexpr uint32_t OFFSET = std::is_same<T, __half>::value ? 0xce00ce00u : 0xc308c308u;  // -24, -136 twice
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   launch_dependents();
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2) int4_few_kernel(const FewArgs p
       slot = (slot + 1) % FW_AHEAD;
 #pragma unroll
       for (int i = 0; i < SUBS; ++i) {
-        float start[4];  // - (B + 8) sum x, by token column
+        float start[4];  // -(B + 8) sum x, by token column
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         const uint32_t offset[4] = {OFFSET, OFFSET, OFFSET, OFFSET};
 #pragma unroll

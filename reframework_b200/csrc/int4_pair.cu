@@ -486,6 +486,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < SUBS; ++i) sc[r][i] = ld_shared_u32(ss + (uint32_t)(i * 4));
       }
+      // a proxy fence before the release: copies of the async proxy refill the
+      // slot, and without it they overtook reads still under way (the last
+      // block's 16 rows came out wrong in most runs of 4096 tokens and more)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(CEMPTY(slot));  // the codes are in registers
       // 16-bit values of rows g (v[..][0]) and g + 8, before the wait: only

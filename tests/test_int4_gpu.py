@@ -180,6 +180,16 @@ def test_repeats_bit_for_bit_and_two_streams(T):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("T,E,top_k,H,I", [(2048, 16, 6, 2048, 1408), (1500, 8, 2, 4096, 2048)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_repeats_bit_for_bit(T, E, top_k, H, I, dtype):
+    """Many tiles a CTA pair, the rings of codes and tokens always full: every run gives the same bits, and the right ones."""
+    x, q1, q2, w, ids = _case(T, E, top_k, H, I, 128, 128, dtype, 30)
+    want, w1, w2 = _check(x, q1, q2, w, ids, 128, 128)
+    outs = [K.moe_experts_int4(x, w1, w2, w, ids) for _ in range(24)]
+    assert [int((o != want).sum()) for o in outs] == [0] * 24
+
+
 @pytest.mark.parametrize("T", [1, 64, 500])
 def test_captured_and_replayed(T):
     x, q1, q2, w, ids = _case(T, 8, 2, 512, 256, 128, 128, torch.bfloat16, 26)

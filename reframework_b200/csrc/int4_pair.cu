@@ -16,8 +16,9 @@
 // TMEM lanes, so the epilogue pairs them with one shuffle.
 //
 // Bound by the MMAs with tiles of 256 tokens: a stage of 128 k takes 1024 cycles
-// of them (4096 tokens through eight experts of 4096 x 14336: 1.89 ms in all,
-// 95 % of the measured bf16 peak).  With few tokens a stage takes 800-860 cycles
+// of them (4096 tokens through eight experts of 4096 x 14336: 1.90-1.94 ms in
+// all, 93 % of the measured bf16 peak; 8192 through 64 of 2048 x 1408: 0.74 ms,
+// 71 %, the rest the permutation, the combine and unfilled tiles).  With few tokens a stage takes 800-860 cycles
 // whatever their number: 32 KB of 16-bit rows are written to shared memory and
 // read back, 18 KB of codes pass in and out, about 700 cycles of its bandwidth
 // (16 tokens through the same experts: 0.28 ms, 40 % of the time their codes

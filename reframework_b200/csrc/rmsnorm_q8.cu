@@ -12,7 +12,9 @@
 // two reductions (sum of squares, then max|z|), each output written once.  The
 // sums and z are fp32; the roundings are those of the outputs' types.  A row
 // belongs to TPR threads (a warp, or a small block) with up to four 16-byte
-// vectors each: few threads per barrier, many independent rows per SM.
+// vectors each: few threads per barrier, many independent rows per SM (8192 x
+// 2048 with groups of 128 and the 16-bit row: 33 us, 71 % of the measured HBM
+// rate; 44 with blocks of 256 threads a row, 45 with a warp of eight vectors).
 #include <cuda_fp8.h>
 
 #include "common.cuh"

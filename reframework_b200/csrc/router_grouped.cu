@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(GR_THREADS) router_grouped_kernel(const Groupe
           if (inside(j)) sb[j] = a.select_bias[e0 + j];
       }
 #pragma unroll
-      for (int j = 0; j < NV; ++j) l[j] = (a.sigmoid ? fast_sigmoid(l[j]) : __expf(l[j] - m) * inv) + sb[j];
+      for (int j = 0; j < NV; ++j)  // a place past the lane's experts stays -inf: a group's top-2 sum sees all NV
+        if (inside(j)) l[j] = (a.sigmoid ? fast_sigmoid(l[j]) : __expf(l[j] - m) * inv) + sb[j];
     }
     uint32_t key[NV];
 #pragma unroll

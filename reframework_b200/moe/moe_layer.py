@@ -153,6 +153,12 @@ class Routing:
             raise ValueError(f"scale must be finite, got {self.scale}")
 
 
+def moved_select_bias(bias: Optional[torch.Tensor], fn) -> Optional[torch.Tensor]:
+    """The selection bias where ``fn`` of ``nn.Module._apply`` puts tensors, still fp32: rounded to a 16-bit layer's
+    type with the parameters, it would choose other experts."""
+    return None if bias is None else bias.to(fn(torch.empty(0, dtype=torch.uint8, device=bias.device)).device)
+
+
 def route_tokens(layer, x2: torch.Tensor, gate: torch.Tensor, shared_gate: Optional[torch.Tensor],
                  round_dtype: Optional[torch.dtype], *, ids32: bool, ids64: bool):
     """The layer's routing of ``x2`` (``kernels.router_topk``'s outputs), by its ``routing`` options if set."""
@@ -271,7 +277,10 @@ class FusedMoE(nn.Module):
         if self._int4 is not None:  # codes and scales change device with the layer, never their types
             dev = fn(self._int4[0].data[:0]).device
             self._int4 = (self._int4[0].to(dev), self._int4[1].to(dev))
-        return super()._apply(fn, recurse)
+        moved = moved_select_bias(self.select_bias, fn)
+        super()._apply(fn, recurse)
+        self.select_bias = moved
+        return self
 
     def quantize_experts(self, group_size: int = 128) -> None:
         """Keep the routed experts as 4-bit codes with one scale per ``group_size`` (32, 64 or 128) input

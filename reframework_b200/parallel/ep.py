@@ -44,7 +44,8 @@ from .. import kernels as K
 from .. import _lib as _lib_mod
 from .._lib import ACTIVATIONS, RfMoeError, check, dtype_code, lib, stream_of
 from ..moe.keys import expert_tensor
-from ..moe.moe_layer import FusedMoE, _bank_view, adjacent_router_weights, reference_output, route_tokens
+from ..moe.moe_layer import (FusedMoE, _bank_view, adjacent_router_weights, moved_select_bias, reference_output,
+                             route_tokens)
 from . import dist as _dist
 from .eplb import Placement, place_experts, split_rows
 
@@ -270,7 +271,10 @@ class EPFusedMoE(nn.Module):
                 p.data = self._slot_bank[0][j]
             for j, p in enumerate(self.experts_w2):
                 p.data = self._slot_bank[1][j]
-        return super()._apply(fn, recurse)
+        moved = moved_select_bias(self.select_bias, fn)
+        super()._apply(fn, recurse)
+        self.select_bias = moved
+        return self
 
     @property
     def num_replicas(self) -> int:

@@ -41,7 +41,7 @@ import math
 import time
 from collections import deque
 from dataclasses import dataclass
-from typing import Deque, Dict, List, Optional, Sequence, Tuple
+from typing import Deque, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -187,7 +187,47 @@ def reference_output(out: torch.Tensor, x: torch.Tensor, hidden: int) -> torch.T
     return out.reshape(x.shape[:1] + (hidden,)) if x.dim() > 1 else out
 
 
-class FusedMoE(nn.Module):
+class RoutingOptions:
+    """``set_routing`` and its selection bias, for the layers (which have ``num_experts``, ``top_k``, ``gate``, and the
+    buffer ``select_bias`` and the attribute ``routing``, both None at first)."""
+
+    def set_routing(self, *, scoring: str = "softmax", select_bias: Union[torch.Tensor, None, str] = "keep",
+                    num_groups: int = 1, topk_groups: int = 1, group_score: str = "max", scale: float = 1.0) -> None:
+        """Route by softmax or sigmoid scores: the ``top_k`` largest ``score + select_bias`` among the
+        ``topk_groups`` best of ``num_groups`` groups of consecutive experts; the weights are the scores alone
+        (renormalised by the layer's ``renormalize``) times ``scale``.  ``select_bias`` [E] is a load-balancing
+        bias (-inf closes an expert), copied; without it the layer keeps the one it has, set before or loaded by
+        ``load_state_dict``, and None clears it."""
+        r = Routing(scoring, int(num_groups), int(topk_groups), group_score, float(scale))
+        r.check(self.num_experts, self.top_k)
+        if isinstance(select_bias, str):
+            if select_bias != "keep":
+                raise ValueError(f"select_bias must be a tensor, None or 'keep', got {select_bias!r}")
+        elif select_bias is None:
+            self.select_bias = None
+        else:
+            self._copy_select_bias(select_bias, "select_bias")
+        self.routing = r
+
+    def _copy_select_bias(self, bias: torch.Tensor, what: str) -> None:
+        """Into the buffer that is there, so that a captured forward sees it, like a loaded weight."""
+        if bias.numel() != self.num_experts:
+            raise ValueError(f"{what} must have {self.num_experts} elements, got {tuple(bias.shape)}")
+        with torch.no_grad():
+            if self.select_bias is None:
+                self.select_bias = torch.empty(self.num_experts, dtype=torch.float32, device=self.gate.device)
+            self.select_bias.copy_(bias.detach().reshape(-1))
+
+    def _load_select_bias(self, state_dict: Dict[str, torch.Tensor], key: str) -> None:
+        if key not in state_dict:
+            return
+        self._copy_select_bias(state_dict[key], key)
+        if self.routing is None:
+            logger.warning("%s is loaded, but only set_routing() routes with it; until then the layer's softmax top-k "
+                           "ignores it", key)
+
+
+class FusedMoE(RoutingOptions, nn.Module):
     """A routed MoE block: ``gate`` -> top-k -> grouped expert GEMMs -> combine."""
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
@@ -256,19 +296,6 @@ class FusedMoE(nn.Module):
         """Add a fixed per-expert bias [E] to the router logits (None clears it)."""
         self.router_bias = None if bias is None else bias.detach().float().to(self.gate.device)
 
-    def set_routing(self, *, scoring: str = "softmax", select_bias: Optional[torch.Tensor] = None, num_groups: int = 1,
-                    topk_groups: int = 1, group_score: str = "max", scale: float = 1.0) -> None:
-        """Route by softmax or sigmoid scores: the ``top_k`` largest ``score + select_bias`` among the
-        ``topk_groups`` best of ``num_groups`` groups of consecutive experts; the weights are the scores alone
-        (renormalised by the layer's ``renormalize``) times ``scale``.  ``select_bias`` [E] is a load-balancing
-        bias (-inf closes an expert)."""
-        r = Routing(scoring, int(num_groups), int(topk_groups), group_score, float(scale))
-        r.check(self.num_experts, self.top_k)
-        if select_bias is not None:
-            if select_bias.numel() != self.num_experts:
-                raise ValueError(f"select_bias must have {self.num_experts} elements, got {tuple(select_bias.shape)}")
-            select_bias = select_bias.detach().reshape(-1).float().to(self.gate.device)
-        self.routing, self.select_bias = r, select_bias
 
     # ------------------------------------------------------------ weight banks
     def _apply(self, fn, recurse=True):
@@ -671,9 +698,7 @@ class FusedMoE(nn.Module):
             g = f"{pre}gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
-            b = f"{pre}gate.e_score_correction_bias"
-            if b in state_dict and self.routing is not None:
-                self.select_bias = state_dict[b].detach().reshape(-1).float().to(self.gate.device)
+            self._load_select_bias(state_dict, f"{pre}gate.e_score_correction_bias")
             I = self.intermediate_size
             for e in range(len(self.experts_w1)):
                 p = f"{pre}experts.{e}"

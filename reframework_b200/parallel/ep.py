@@ -44,8 +44,8 @@ from .. import kernels as K
 from .. import _lib as _lib_mod
 from .._lib import ACTIVATIONS, RfMoeError, check, dtype_code, lib, stream_of
 from ..moe.keys import expert_tensor
-from ..moe.moe_layer import (FusedMoE, _bank_view, adjacent_router_weights, moved_select_bias, reference_output,
-                             route_tokens)
+from ..moe.moe_layer import (FusedMoE, RoutingOptions, _bank_view, adjacent_router_weights, moved_select_bias,
+                             reference_output, route_tokens)
 from . import dist as _dist
 from .eplb import Placement, place_experts, split_rows
 
@@ -159,7 +159,7 @@ def plan_dispatch(counts_all: np.ndarray, rank: int, shards: Sequence[Tuple[int,
     return plan_exchange(counts_all, rank, placement, None, align)
 
 
-class EPFusedMoE(nn.Module):
+class EPFusedMoE(RoutingOptions, nn.Module):
     """Expert-sharded MoE layer with the same forward / state-dict contract as
     the reference ``EPFusedMoE`` (ep.py:58-179)."""
 
@@ -195,7 +195,7 @@ class EPFusedMoE(nn.Module):
         self.experts_w2 = nn.ParameterList([nn.Parameter(w2[j]) for j in range(n)])
         self.register_buffer("router_bias", None, persistent=False)
         self.register_buffer("select_bias", None, persistent=False)
-        self.routing = None  # FusedMoE.set_routing's options, from the sharded layer
+        self.routing = None  # set_routing's options, its own or the sharded layer's
         self.entropy_adaptive_k = False
         self.entropy_k_min = 2
         self.precise_combine = False
@@ -250,7 +250,8 @@ class EPFusedMoE(nn.Module):
                 b1.copy_(w1b[ep.local_start:ep.local_end])
                 b2.copy_(w2b[ep.local_start:ep.local_end])
         ep.router_bias = base.router_bias
-        ep.routing, ep.select_bias = base.routing, base.select_bias
+        ep.routing = base.routing
+        ep.select_bias = None if base.select_bias is None else base.select_bias.clone()
         ep.entropy_adaptive_k = base.entropy_adaptive_k
         ep.entropy_k_min = base.entropy_k_min
         ep.precise_combine = base.precise_combine
@@ -825,9 +826,7 @@ class EPFusedMoE(nn.Module):
             g = f"{pre}gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
-            b = f"{pre}gate.e_score_correction_bias"
-            if b in state_dict and self.routing is not None:
-                self.select_bias = state_dict[b].detach().reshape(-1).float().to(self.gate.device)
+            self._load_select_bias(state_dict, f"{pre}gate.e_score_correction_bias")
             I = self.intermediate_size
             for j, gg in enumerate(range(self.local_start, self.local_end)):
                 p = f"{pre}experts.{gg}"

@@ -37,3 +37,57 @@ def test_a_layer_cast_to_another_type_keeps_its_selection_bias(cast):
         assert layer.select_bias.dtype == torch.float32 and torch.equal(layer.select_bias, _bias())
     assert "select_bias" in dict(moe.named_buffers())
     assert moe.to("meta").select_bias.is_meta
+
+
+@pytest.mark.parametrize("make", [_fused, _sharded])
+@pytest.mark.parametrize("prefix", ["", "layers.3.mlp"])
+def test_the_bias_is_loaded_whatever_the_order(make, prefix, caplog):
+    src = make()
+    src.set_routing(scoring="sigmoid", select_bias=_bias())
+    saved = {k: v.clone() for k, v in src.state_dict(prefix=prefix).items()}
+    before, after = make(), make()
+    before.set_routing(scoring="sigmoid")
+    before.load_state_dict(saved, prefix=prefix)
+    assert not caplog.records
+    after.load_state_dict(saved, prefix=prefix)
+    assert after.routing is None and "set_routing" in caplog.text  # loaded, not in use yet: said so
+    after.set_routing(scoring="sigmoid")
+    for layer in (before, after):
+        assert layer.routing.scoring == "sigmoid" and torch.equal(layer.select_bias, _bias())
+        assert layer.select_bias.dtype == torch.float32
+
+
+@pytest.mark.parametrize("make", [_fused, _sharded])
+def test_set_routing_keeps_replaces_and_clears_the_bias(make):
+    layer, b = make(), _bias()
+    layer.set_routing(select_bias=b)
+    at = layer.select_bias.data_ptr()
+    b.zero_()  # copied
+    layer.set_routing(scoring="sigmoid", num_groups=2, topk_groups=1)
+    assert torch.equal(layer.select_bias, _bias()) and layer.routing.num_groups == 2
+    layer.set_routing(select_bias=b.double())
+    assert torch.equal(layer.select_bias, b) and layer.select_bias.data_ptr() == at
+    with pytest.raises(ValueError, match="select_bias"):
+        layer.set_routing(select_bias="drop")
+    assert layer.routing.scoring == "softmax"
+    layer.set_routing(select_bias=None)
+    assert layer.select_bias is None
+
+
+@pytest.mark.parametrize("make", [_fused, _sharded])
+@pytest.mark.parametrize("routed", [False, True])
+def test_a_bias_of_another_length_is_refused(make, routed):
+    layer = make()
+    if routed:
+        layer.set_routing(scoring="sigmoid", select_bias=_bias())
+    with pytest.raises(ValueError, match="e_score_correction_bias must have 8 elements"):
+        layer.load_state_dict({"gate.e_score_correction_bias": torch.zeros(E + 1)})
+    assert (torch.equal(layer.select_bias, _bias()) if routed else layer.select_bias is None)
+
+
+def test_a_sharded_layer_has_its_own_bias():
+    moe = _fused()
+    moe.set_routing(scoring="sigmoid", select_bias=_bias())
+    ep = EPFusedMoE.from_full(moe, 1, 0)
+    moe.select_bias.zero_()
+    assert torch.equal(ep.select_bias, _bias())

@@ -130,3 +130,20 @@ def test_inputs_stay_and_graph_replays():
         got = K.add_rmsnorm_q8(x, w, residual=r, group_size=128)
     graph.replay()
     assert torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(got.scales, want.scales)
+
+
+@pytest.mark.parametrize("T,H", [(3, 64), (5, 512), (64, 4096), (700, 1024), (400, 6144)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_the_sum_in_place_of_an_input(T, H, dtype, over):
+    """The library call with residual_out = x or = residual: the same bits as with an output of its own."""
+    x, w, r, _ = _inputs(T, H, dtype, T, True, False)
+    want = K.add_rmsnorm_q8(x, w, residual=r, group_size=32, want_normed=True)
+    q, scales, normed = torch.empty_like(want.q), torch.empty_like(want.scales), torch.empty_like(x)
+    out = {"x": x, "residual": r}[over]
+    rc = _lib.lib().rf_moe_add_rmsnorm_q8(x.data_ptr(), r.data_ptr(), T, H, _lib.dtype_code(dtype), w.data_ptr(), None, 1e-6, 32,
+                                          out.data_ptr(), normed.data_ptr(), q.data_ptr(), scales.data_ptr(),
+                                          _lib.stream_of(x.device))
+    assert rc == 0
+    assert torch.equal(out, want.residual) and torch.equal(normed, want.normed)
+    assert torch.equal(q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(scales, want.scales)

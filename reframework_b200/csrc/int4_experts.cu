@@ -502,14 +502,15 @@ __global__ void __launch_bounds__(CB_THREADS) int4_combine_kernel(const CombineA
     }
     const int64_t at = t * a.H + col;
     float f[8];
+    // ordinary loads, not the read-only path: out may be residual
     if (a.shared_y) {
-      rf::unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.shared_y) + at)), f);
+      rf::unpack16<T>(__ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.shared_y) + at)), f);
       const float s = a.shared_scale ? a.shared_scale[t] : 1.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = fmaf(s, f[i], acc[i]);
     }
     if (a.residual) {
-      rf::unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.residual) + at)), f);
+      rf::unpack16<T>(__ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.residual) + at)), f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] += f[i];
     }

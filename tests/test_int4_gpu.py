@@ -243,3 +243,18 @@ def test_scales_with_all_their_bits(T, impl):
         dh = u * (1.2 * mag[:, :128] * (up.abs() + u * mag[:, 128:]) + a.abs() * mag[:, 128:])
         extra.index_add_(0, t, wk * (((1 + 2 * u) * dh + u * (a * up).abs()) @ d2[e].abs().T))
     assert bool(((out.double() - ref).abs() <= bound + (1 + u) * extra).all())
+
+
+@pytest.mark.parametrize("T", [1, 7, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("over", ["residual", "shared_y", "x"])
+def test_the_output_in_place_of_an_input(T, dtype, over):
+    """out may be one of the call's own rows: the same bits as with an output of its own."""
+    x, q1, q2, w, ids = _case(T, 8, 2, 256, 128, 128, 64, dtype, 31)
+    g = torch.Generator().manual_seed(2)
+    sy, res = (torch.randn(T, 256, generator=g).to(dtype).to(DEV) for _ in range(2))
+    w1, w2 = K.int4_pack(*q1, group_size=128, gated=True), K.int4_pack(*q2, group_size=64)
+    want = K.moe_experts_int4(x, w1, w2, w, ids, shared_y=sy, residual=res)
+    out = {"residual": res, "shared_y": sy, "x": x}[over]
+    got = K.moe_experts_int4(x, w1, w2, w, ids, shared_y=sy, residual=res, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)

@@ -20,11 +20,10 @@
 // a gated weight's gate and up halves are padded to whole row blocks each.
 #pragma once
 
-#include <map>
-#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.cuh"
 
 namespace rf {
 
@@ -93,24 +92,10 @@ template <> __device__ __forceinline__ uint32_t int4_pair<__half>(uint32_t word,
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// What a kernel's set-up found on each device (function attributes are a
-// device's own): `find` runs once per device, on the current one; 0: it failed.
-class PerDevice {
- public:
-  template <typename F>
-  int get(F find) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    std::lock_guard<std::mutex> lock(mu_);
-    auto it = found_.find(dev);
-    if (it == found_.end()) it = found_.emplace(dev, find()).first;
-    return it->second;
-  }
-
- private:
-  std::mutex mu_;
-  std::map<int, int> found_;
-};
+inline int current_device() {
+  int dev = -1;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
 
 // One grouped product over all experts, rows in permuted order.
 struct Int4Gemm {

@@ -423,7 +423,7 @@ int launch_few_k(FewArgs p, cudaStream_t st) {
   auto kern = int4_few_kernel<T, GATED, SUBS, KS>;
   const char *what = GATED ? "4-bit gated products (few rows)" : "4-bit down products (few rows)";
   static rf::PerDevice fit;
-  const int resident = fit.get([&]() -> int {
+  const int resident = fit.get(rf::current_device(), [&]() -> int {
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FewShared)) != cudaSuccess) return 0;
     return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, FW_THREADS, sizeof(FewShared)) == cudaSuccess ? n : 0;

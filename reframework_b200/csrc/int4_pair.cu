@@ -556,7 +556,7 @@ template <typename T, bool GATED, int SUBS>
 int launch_pair_t(const TokMaps &mx, const CUtensorMap &mw, const CUtensorMap &ms, const PairArgs &p, cudaStream_t st) {
   auto kern = int4_pair_gemm<T, GATED, SUBS>;
   static rf::PerDevice fit;
-  const int clusters = fit.get([&]() -> int {
+  const int clusters = fit.get(rf::current_device(), [&]() -> int {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q_SMEM_BYTES) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * std::max(1, rf::num_sms() / 2), 1, 1);

@@ -15,7 +15,12 @@
 // are picked by fp32 values with a bound on their error, and where a decision
 // hangs on a gap within that bound the candidates are put in order by their
 // fp64 scores (without a bias c is monotone in l, so logits are compared then).
-// The weights are computed from the chosen logits alone, to full fp32 accuracy.
+// The weights are computed again from the chosen logits, with expf.  A softmax
+// score is then divided by the sum over all experts, which is one of __expf.  A
+// term e^-d of it, d = m - l, is off by (2 + 1.173 d + d / 2) * 2^-23 of itself,
+// and the mean of d over a softmax is at most ln E, so the sum is off by at most
+// (27.2 + NV + 5) * 2^-24 of itself (E = 1024; NV + 5 additions).  A score is that
+// and d + 5 roundings off; renormalised, the sum cancels and d + 5 twice stay.
 //
 // One warp per token: lane i holds the nv consecutive experts from i * nv as
 // order-preserving integer keys, sorted, nv being a divisor of the group size

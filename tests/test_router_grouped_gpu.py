@@ -184,3 +184,24 @@ def test_on_a_side_stream_and_in_a_graph():
     graph.replay()
     want = K.router_grouped_topk(l, None, 6, scoring="sigmoid")
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("T,E,top_k", [(300, 8, 2), (300, 64, 6), (500, 256, 8), (200, 1000, 16), (100, 1024, 16)])
+@pytest.mark.parametrize("spread", [0.01, 1.5, 8.0])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_how_near_softmax_weights_come(T, E, top_k, spread, renormalize):
+    """With d = max - l: a score e^-d / sum has an expf of at most 2 ulp (4 * 2^-24) whose argument is rounded (d * 2^-24)
+    and a division; the sum is off by 2 + 1.673 * mean(d) ulp, mean(d) <= ln E over a softmax, and by its NV + 5
+    additions, NV <= 32 the power of two from E / 32 on.  Renormalised, the sum cancels, and each of the two sides has
+    d + 5, the second also four additions, a division and the scale's product."""
+    l = _logits(T, E, torch.float32, E) * (spread / 1.5)
+    w, ids, _, _, _ = K.router_grouped_topk(l, None, top_k, renormalize=renormalize)
+    rw, rids = R.route(l, top_k, scoring="softmax", renormalize=renormalize)
+    assert torch.equal(ids.long(), rids)
+    d = (l.amax(1, keepdim=True) - torch.gather(l, 1, rids)).double()
+    nv = 1
+    while 32 * nv < E:
+        nv *= 2
+    of_sum = 2 * (2 + 1.673 * math.log(E)) + nv + 5
+    steps = 2 * (d.amax(1, keepdim=True) + 5) + 6 if renormalize else of_sum + d + 5 + 1
+    assert bool(((w.double() - rw).abs() <= steps * 2.0 ** -24 * rw + 2.0 ** -149).all())

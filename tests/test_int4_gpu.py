@@ -258,3 +258,43 @@ def test_the_output_in_place_of_an_input(T, dtype, over):
     out = {"residual": res, "shared_y": sy, "x": x}[over]
     got = K.moe_experts_int4(x, w1, w2, w, ids, shared_y=sy, residual=res, out=out)
     assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind,size", [("codes near 8", 1.0), ("closed channels", 100.0), ("closed channels", 1000.0),
+                                       ("closed channels", 50000.0)])
+@pytest.mark.parametrize("impl", [1, 5])
+def test_where_the_offset_of_the_codes_cancels_most(group, dtype, kind, size, impl):
+    """x of one sign with codes 7..9, and huge channels whose codes are all 8, which add nothing.  The few-row kernel's
+    codes carry an offset B: a group's sum is off by up to F = 4 * PER * 17 * 2^-23 * (B + 15) of scale * sum |x|
+    beyond R.experts' bound (PER = group / 32; derived at the kernel); the CTA-pair kernel's codes carry none."""
+    _lib.set_gemm_impl(impl)
+    T, E, H, I = 6, 2, 512, 256
+    x, (c1, s1), (c2, s2), w, ids = _case(T, E, 1, H, I, group, group, dtype, 33)
+    if kind == "codes near 8":
+        q = torch.randint(7, 10, (E, 2 * I, H), generator=torch.Generator().manual_seed(5), dtype=torch.uint8)
+        c1 = (q[..., 0::2] | (q[..., 1::2] << 4)).to(DEV)
+        x = x.abs()
+    else:
+        c1[:, :, 2] = (c1[:, :, 2] & 0x0f) | 0x80       # k = 5
+        c1[:, :, 128] = (c1[:, :, 128] & 0xf0) | 0x08   # k = 256
+        x[:, 5], x[:, 256] = size, -size
+    w1, w2 = K.int4_pack(c1, s1, group_size=group, gated=True), K.int4_pack(c2, s2, group_size=group)
+    out = K.moe_experts_int4(x, w1, w2, w, ids)
+    d1, d2 = R.dequantise(c1, s1, group), R.dequantise(c2, s2, group)
+    ref, bound = R.experts(x, d1, d2, w, ids, "silu")
+    if impl == 1:
+        f = 4 * (group // 32) * 17 * 2.0 ** -23 * ((16 if dtype == torch.float16 else 128) + 15)
+        u = torch.finfo(dtype).eps / 2
+        for t in range(T):
+            e = int(ids[t, 0])
+            g, up = (d1[e] @ x[t].double()).view(2, I)
+            extra = f * (s1[e].double() @ x[t].double().abs().view(-1, group).sum(1)).view(2, I)
+            h = R.act("silu", g) * up
+            # |act'| < 1.2, as in R.experts; its own bounds of g and u, eg and eu, are below 2^-7 of |x||w|
+            mag = (d1[e].abs() @ x[t].double().abs()).view(2, I) * H * 2.0 ** -23
+            dh = 1.2 * extra[0] * (up.abs() + extra[1] + mag[1]) + (R.act("silu", g).abs() + 1.2 * mag[0]) * extra[1]
+            most = h.abs() + dh * 2 + u
+            bound[t] += (1 + 4 * u) * (d2[e].abs() @ dh + f * s2[e].double() @ most.view(-1, group).sum(1))
+    assert bool(((out.double() - ref).abs() <= bound).all())

@@ -313,7 +313,8 @@ class FusedMoE(RoutingOptions, nn.Module):
         """Keep the routed experts as 4-bit codes with one scale per ``group_size`` (32, 64 or 128) input
         features (``kernels.int4_quantize``) and free their 16-bit weights.  The layer must be on its CUDA
         device, resident (no offload cache) and of a 16-bit dtype; the router and the shared experts stay as they
-        are.  ``state_dict`` then returns the dequantised experts; ``load_state_dict`` comes before."""
+        are.  ``state_dict`` then returns the dequantised experts; ``load_state_dict`` comes before.  A CUDA
+        graph captured before still reads the 16-bit weights, which are freed here: capture the quantised layer."""
         if self.uses_offload:
             raise RfMoeError("quantize_experts: the experts are offloaded; quantise a resident layer")
         if self._int4 is not None:

@@ -192,3 +192,19 @@ def test_offloaded_layer_routes_in_groups():
         assert torch.equal(moe.route(x)[1], ids)
         got = moe(x)
     torch.testing.assert_close(got.float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -8 * float(want.abs().max()))
+
+
+def test_a_captured_layer_routes_with_the_bias_set_or_loaded_later():
+    moe = _layer(seed=21)
+    graph = capture_forward(moe, _x(20, 1))
+    x = _x(20, 2)
+    for seed, loads in ((1, False), (2, True)):
+        b = torch.randn(E, generator=torch.Generator().manual_seed(seed)) * 0.3
+        before = graph(x).clone()
+        if loads:
+            moe.load_state_dict({"gate.e_score_correction_bias": b})
+        else:
+            moe.set_routing(scoring="sigmoid", select_bias=b, num_groups=4, topk_groups=2, group_score="top2", scale=2.5)
+        with torch.no_grad():
+            want = moe(x)
+        assert torch.equal(graph(x), want) and not torch.equal(want, before)

@@ -621,6 +621,12 @@ int rf_moe_int4_dequantize(const void *data, const void *packed_scales, int dtyp
  * w1 a gated weight of N = 2I, K = H, w2 one of N = H, K = I, E slots each;
  * topk_ids outside [0, E) add nothing and set RF_DEV_BAD_EXPERT_ID.
  * shared_y, shared_scale, residual may be NULL; out may be residual.
+ * h is rounded to dtype (past 65504 an fp16 h is infinite).  Two kernels, by the
+ * number of pairs (T * K) and rows an expert: the one for many rows rounds
+ * scale * (code - 8) to dtype, which is exact for scales of up to five
+ * significant bits, as rf_moe_int4_quantize's; the one for few rows (up to 1024
+ * pairs, fewer than 9 an expert) does not, but its fp32 sums are off by a
+ * multiple of sum |x|, codes of 8 included.
  * workspace: rf_moe_int4_experts_workspace_size bytes, 256-byte aligned.
  */
 size_t rf_moe_int4_experts_workspace_size(int64_t T, int64_t K, int64_t E, int64_t H, int64_t I);

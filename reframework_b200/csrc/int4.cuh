@@ -65,15 +65,18 @@ inline bool int4_valid(int64_t N, int64_t K, int64_t group, bool gated) {
 }
 
 // The pair of codes (2 i, 2 i + 1) of a word as two 16-bit values code + B,
-// exact.  bf16: the last mantissa bits of 128.0, B = 128.  fp16: the first ones
-// of 16.0, B = 16, a shift more: the last bits of 1024.0 made a product's terms
-// 40 times as large, and an fp16 layer came out off by 0.00033, not 0.00029.
+// exact, by placing the codes in the mantissas of B (published by Kim, Henry,
+// Fahim and Awadalla, "Who Says Elephants Can't Run", 2022, with the order of the
+// codes that it needs).  bf16: the last mantissa bits of 128.0, B = 128.  fp16:
+// the first ones of 16.0, B = 16, a shift more: the last bits of 1024.0 made a
+// product's terms 40 times as large, and an fp16 layer came out off by 0.00033,
+// not 0.00029.
 template <typename T> __device__ __forceinline__ uint32_t int4_raw(uint32_t word, int i) {
   constexpr bool HALF = std::is_same<T, __half>::value;
   constexpr int AT = HALF ? 6 : 0;  // the code's place in the mantissa
   constexpr uint32_t MASK = 0x000f000fu << AT, BASE = HALF ? 0x4c004c00u : 0x43004300u;
   const uint32_t w = 4 * i < AT ? word << (AT - 4 * i) : word >> (4 * i - AT);
-  uint32_t r;  // (word & mask) | base in one instruction: written in C it became two
+  uint32_t r;  // (word & mask) | base; in C++ 7 tokens through eight experts of 4096 x 14336 took 178 us, so 144
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(MASK), "r"(BASE));
   return r;
 }

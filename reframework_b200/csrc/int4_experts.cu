@@ -19,9 +19,9 @@
 // ids, h and y rows are the pairs themselves, and the three launches (gated,
 // down, combine) are chained by programmatic dependent launch, each waiting for
 // its predecessor's rows only after its ids and first weights are on the way.
-// Measured: 7 tokens through eight experts of 4096 x 14336 144 us (73 % of the
-// measured HBM rate), one token 58 us; 64 tokens through 60 experts of 2048 x
-// 1408 85 us, one token 15 us.
+// Measured: 7 tokens through eight experts of 4096 x 14336, groups of 32, 146 us
+// where they reach six experts, 178 at 7.3 (62 % of the measured HBM rate), one
+// token 58 us; 64 tokens through 60 experts of 2048 x 1408 85 us, one token 15 us.
 // Many rows per expert: permute with the row gather, then int4_pair.cu.
 #include <algorithm>
 #include <string>
@@ -36,12 +36,16 @@ namespace {
 
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = FW_WARPS * 32;
-constexpr int FW_PAIRS = 1024;  // pairs that a block's list holds
+// Pairs that a block's list holds; more take the CTA-pair kernel whatever their
+// rows.  Not a crossover: 256 experts of 2048 x 512, 4 rows each (1024 pairs) 133 us
+// here, 199 there; 5 and 8 rows (1280, 2048 pairs) take 202 and 204 there.
+constexpr int FW_PAIRS = 1024;
 constexpr int FW_STEP = rf::I4_STEP;
 constexpr int FW_AHEAD = 4;     // a power of two: ring slots of a warp: steps of codes on their way, and the one in use
-// 32-row units from which two warps share a unit's k instead of eight: longer
-// runs per job (64 tokens through 60 experts: 111 -> 101 us), while below it jobs
-// of four units would leave blocks idle.
+// 32-row units (times experts) from which two warps share a unit's k instead of
+// eight: longer runs per job, while below it jobs of four units would leave blocks
+// idle (2368 units are two jobs for each of 296 resident blocks).  Measured at one
+// shape: 64 tokens through 60 experts of 2048 x 1408, 111 us with eight, 101 with two.
 constexpr int FW_MANY_JOBS = 2368;
 constexpr int KMAX = 16;
 

@@ -16,22 +16,23 @@
 // TMEM lanes, so the epilogue pairs them with one shuffle.
 //
 // Bound by the MMAs with tiles of 256 tokens: a stage of 128 k takes 1024 cycles
-// of them (4096 tokens through eight experts of 4096 x 14336: 1.90-1.94 ms in
-// all, 93 % of the measured bf16 peak; 8192 through 64 of 2048 x 1408: 0.74 ms,
-// 71 %, the rest the permutation, the combine and unfilled tiles).  With few tokens a stage takes 800-860 cycles
+// of them (4096 tokens through eight experts of 4096 x 14336: 1.91-1.93 ms in
+// all, 93 % of the measured bf16 peak, 2.21 in a steady run at the power cap;
+// 8192 through 64 of 2048 x 1408: 0.73 ms, 72 %, the rest the permutation, the
+// combine and unfilled tiles).  With few tokens a stage takes 800-860 cycles
 // whatever their number: 32 KB of 16-bit rows are written to shared memory and
 // read back, 18 KB of codes pass in and out, about 700 cycles of its bandwidth
-// (16 tokens through the same experts: 0.28 ms, 40 % of the time their codes
-// take from memory).  Tried without gain there: a ring of tokens of its own, two
-// slots of codes per stage, 24 code warps, codes called into L2 ahead.
+// (16 tokens through the same experts: 0.28 ms, 40 % of the HBM rate).  Tried
+// without gain there: a ring of tokens of its own, two slots of codes per stage,
+// 24 code warps, codes called into L2 ahead.
 //
-// Roles (a cluster of two CTAs per pair, persistent, 14 warps):
+// Roles (a cluster of two CTAs per pair, persistent, 19 warps):
 //   warp 0        TMA producer of this CTA's token rows
 //   warp 1        first CTA: MMA issuer
 //   warps 2-5     epilogue, one per TMEM lane quadrant
 //   warps 6-17    codes -> 16-bit rows: four warps (32 rows each) for each of
-//                 the ring's three slots, so that three stages are in work at
-//                 a time; each warp copies its own codes, one use ahead
+//                 the ring's three slots, so that three stages are in work at a time
+//   warp 18       TMA producer of this CTA's codes and scales
 // A stage of the ring holds 128 k: it is full when the token bytes of both CTAs
 // and the arrivals of the pair's eight code warps of its slot are in, and empty when
 // the MMAs that read it have committed.  Tiles (group, feature block, token
@@ -96,8 +97,7 @@ struct TokMaps {
 // over stays on this SM: rows in this CTA's shared memory that this SM's tensor
 // core reads (ordered by the proxy fence before it), or this CTA's TMEM; only
 // the count is kept by the other CTA.  A release of cluster scope here waited
-// 1000-1800 cycles, once per stage (measured with clock64 on C2's shapes: the
-// stage period fell from 1760 cycles with it).
+// 1000-1800 cycles, once per stage (clock64, eight experts of 4096 x 14336).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -323,8 +323,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1)
     if (rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       // The whole warp walks the loop and one elected lane issues: addresses
-      // and descriptors stay warp-uniform (inside a one-lane branch an MMA took
-      // 88 cycles to issue, most of it moving its operands to uniform registers).
+      // and descriptors stay warp-uniform (inside a one-lane branch an MMA took 88
+      // cycles to issue; 16 tokens: 0.42 -> 0.29 ms).
       const uint32_t IDESC = pair_idesc_base<T>();
       const uint32_t peer_bars = mapa_shared(bar0, 1);
       const uint32_t a_desc = sw128_desc_lo(smem_u32(sA)), b_desc = sw128_desc_lo(smem_u32(sB));

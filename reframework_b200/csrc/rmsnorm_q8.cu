@@ -8,13 +8,14 @@
 // An all-zero group has scale 1; a group holding a NaN or an infinity has
 // scale NaN and zero codes, so that every value it stands for is NaN.
 //
-// HBM-bound: each input element is read once and kept in registers across the
-// two reductions (sum of squares, then max|z|), each output written once.  The
-// sums and z are fp32; the roundings are those of the outputs' types.  A row
-// belongs to TPR threads (a warp, or a small block) with up to four 16-byte
-// vectors each: few threads per barrier, many independent rows per SM (8192 x
-// 2048 with groups of 128 and the 16-bit row: 33 us, 71 % of the measured HBM
-// rate; 44 with blocks of 256 threads a row, 45 with a warp of eight vectors).
+// Each input element is read once and kept in registers across the reductions (sum
+// of squares, then max|z|), each output written once.  The sums and z are fp32; the
+// roundings are those of the outputs' types.  A row belongs to TPR threads (a warp,
+// or a small block) with up to four 16-byte vectors each: few threads per barrier,
+// many independent rows per SM.  A block has nothing on its way behind its own
+// row's loads: 8192 x 2048 with groups of 128 and the 16-bit row takes 31.5-33 us,
+// 70-74 % of the measured HBM rate (one barrier a row, 3.5 waves of blocks, issue
+// slots 64 % busy); blocks of 256 threads a row took 44, a warp of eight vectors 45.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -219,7 +220,8 @@ int launch_v(const NormArgs &a, cudaStream_t st) {
 
 // Few rows leave SMs idle, so a row gets twice the threads (64 rows of 4096:
 // 3.5 us against 4.2); with many, four vectors a thread keep more bytes in
-// flight for each barrier (2047 rows of 6144: 15.8 us against 19.1).
+// flight for each barrier (2047 rows of 6144: 15.8 us against 19.1; 16.4-17.4
+// with inputs from HBM: two barriers a row, 2.8 waves).
 template <typename T>
 int launch_t(const NormArgs &a, cudaStream_t st) {
   const int nvec = a.H / (16 / (int)sizeof(T));

@@ -29,10 +29,11 @@
 // redux.sync over the lanes' first keys and a shift in the lane that had it.
 // The place within a lane is kept in a key's low bits (part of the error
 // bound).  Sizes without such an nv, e.g. groups of 37, take an fp64 form.
-// Bound by issuing instructions: about 1250 a token for 256 experts and K = 8
-// in 8 groups, of which 8 sigmoids a lane, a sort of 8 and 13 picks or
-// reductions: 8192 such tokens take 18 us (their bytes alone 1.4), one of 64
-// experts 4.2 us, nearly all of it the launch.
+// Bound by latency: a chain of dependent reductions per pick, 6.8 warps a
+// scheduler (64 registers: 8 blocks an SM, 1.73 waves of 8192 tokens), issue slots
+// 46 % busy.  256 experts, K = 8, 8 groups: 1263 instructions a token, of which 8
+// sigmoids a lane, a sort of 8 and 13 picks or reductions; 8192 tokens take 18 us
+// (their bytes alone 1.4), one of 64 experts 3.8, nearly all of it the launch.
 #include "router.cuh"
 
 namespace {

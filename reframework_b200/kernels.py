@@ -530,7 +530,9 @@ def moe_experts_int4(x: torch.Tensor, w1: Int4Weights, w2: Int4Weights, weights:
                      shared_scale: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`moe_experts` with 4-bit weights (routing given): permute, gated products, down products and
-    an fp32 combine rounded once, ``out[t] = sum_k w[t,k] y + shared_scale * shared_y + residual``."""
+    an fp32 combine rounded once, ``out[t] = sum_k w[t,k] y + shared_scale * shared_y + residual``.
+    ``out`` may be ``x``, ``residual`` or ``shared_y``.  Scales of more than five significant bits (a checkpoint's, through
+    :func:`int4_pack`) are rounded into the weights where experts have many rows, and not where they have few."""
     dev = _require_cuda(x, w1.data, w2.data, weights, ids32, shared_y, shared_scale, residual, out)
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"unknown gated activation {activation!r}; known: {tuple(_lib.ACTIVATIONS)}")

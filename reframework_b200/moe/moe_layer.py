@@ -214,7 +214,8 @@ class RoutingOptions:
         if bias.numel() != self.num_experts:
             raise ValueError(f"{what} must have {self.num_experts} elements, got {tuple(bias.shape)}")
         with torch.no_grad():
-            if self.select_bias is None:
+            old = self.select_bias
+            if old is None or old.is_inference() > torch.is_inference_mode_enabled():  # else it cannot be written
                 self.select_bias = torch.empty(self.num_experts, dtype=torch.float32, device=self.gate.device)
             self.select_bias.copy_(bias.detach().reshape(-1))
 

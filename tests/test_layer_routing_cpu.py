@@ -91,3 +91,15 @@ def test_a_sharded_layer_has_its_own_bias():
     ep = EPFusedMoE.from_full(moe, 1, 0)
     moe.select_bias.zero_()
     assert torch.equal(ep.select_bias, _bias())
+
+
+def test_a_bias_set_in_inference_mode_can_be_replaced_outside():
+    moe = _fused()
+    with torch.inference_mode():
+        moe.set_routing(scoring="sigmoid", select_bias=_bias())
+        moe.set_routing(select_bias=_bias().flip(0))
+    moe.load_state_dict({"gate.e_score_correction_bias": _bias()})
+    assert torch.equal(moe.select_bias, _bias())
+    with torch.inference_mode():
+        moe.load_state_dict({"gate.e_score_correction_bias": _bias().flip(0)})
+    assert torch.equal(moe.select_bias, _bias().flip(0))

@@ -620,7 +620,7 @@ int rf_moe_int4_dequantize(const void *data, const void *packed_scales, int dtyp
  * x [T, H], out / shared_y / residual [T, H] in dtype (RF_BF16 or RF_F16);
  * w1 a gated weight of N = 2I, K = H, w2 one of N = H, K = I, E slots each;
  * topk_ids outside [0, E) add nothing and set RF_DEV_BAD_EXPERT_ID.
- * shared_y, shared_scale, residual may be NULL; out may be residual.
+ * shared_y, shared_scale, residual may be NULL; out may be x, residual or shared_y.
  * h is rounded to dtype (past 65504 an fp16 h is infinite).  Two kernels, by the
  * number of pairs (T * K) and rows an expert: the one for many rows rounds
  * scale * (code - 8) to dtype, which is exact for scales of up to five
